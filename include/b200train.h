@@ -1,0 +1,63 @@
+/*
+ * b200train -- C ABI of the steps of a fine-tuning step that lie between the attention and expert kernels
+ * (b200attn.h, b200moe.h) and the optimizer: the residual sum with its RMS norm, the global gradient norm with
+ * clipping, and the clipped SGD update.  Part of libb200attn.so.
+ *
+ * The reference project leaves them to Hugging Face (GptOssRMSNorm.forward and the two sums of
+ * GptOssDecoderLayer.forward, transformers/models/gpt_oss/modeling_gpt_oss.py:48-63, :357-386) and to its launcher
+ * (gradient clipping at 1.0, configs/zero3.yaml:6).
+ *
+ * Conventions as in b200attn.h: device pointers unless said otherwise, no allocation, no synchronisation, calls only
+ * enqueue work on `stream` of `device`; 0 on success or a negative B200ATTN_E* code (b200attn_strerror explains it).
+ */
+#ifndef B200TRAIN_H_
+#define B200TRAIN_H_
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "b200attn.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Element types. */
+enum { B200TRAIN_BF16 = 0, B200TRAIN_FP16 = 1, B200TRAIN_FP32 = 2 };
+
+#define B200TRAIN_NORM_MAX_COLS 16384 /* widest row of the norm */
+
+/*
+ * h[t,:] = round(x[t,:] + residual[t,:]);  y[t,c] = round(weight[c] * h[t,c] * rsqrt(mean_c(h[t,c]^2) + eps)).
+ * The sum is rounded to the element type first (it is the residual stream), the norm is taken of the rounded row in
+ * fp32 and rounded once.  residual == NULL: h is x itself, and `h` must be NULL too.
+ *   x, residual   (rows x cols), element type `dtype`, element strides x_stride / residual_stride between rows
+ *   weight        (cols), element type `weight_dtype`: `dtype` or B200TRAIN_FP32
+ *   y, h          (rows x cols) contiguous, fully overwritten; neither may overlap an input
+ * Base pointers 16-byte aligned.  Where cols is a multiple of 16 bytes' worth of elements, the strides must be too;
+ * otherwise the inputs must be contiguous (stride == cols).  rows >= 0, 1 <= cols <= B200TRAIN_NORM_MAX_COLS.
+ */
+int b200train_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                           const void* weight, void* y, void* h, int64_t rows, int32_t cols, float eps, int32_t dtype,
+                           int32_t weight_dtype, int32_t device, void* stream);
+
+/* fp32 values of scratch that b200train_add_rms_norm_bwd needs to make dweight (0 where it needs none). */
+int64_t b200train_norm_scratch_floats(int64_t rows, int32_t cols, int32_t dtype, int32_t device);
+
+/*
+ * The gradients of the above: with n = h * rstd, g = dy * weight,
+ *   dx[t,:] = dh[t,:] + rstd * (g - n * mean_c(g * n))      (the gradient of x and of residual alike)
+ *   dweight[c] = sum_t dy[t,c] * n[t,c]                     (fp32, in an order fixed by the sizes)
+ * rstd is taken from h again.  dh may be NULL (no gradient arrives through h); dweight may be NULL (not wanted; scratch
+ * is then not used).  dx (rows x cols) contiguous, dweight (cols) of `weight_dtype`, both fully overwritten.
+ * Alignment and strides as above, for dy, dh and h.
+ */
+int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
+                               int64_t h_stride, const void* weight, void* dx, void* dweight, float* scratch,
+                               int64_t scratch_floats, int64_t rows, int32_t cols, float eps, int32_t dtype,
+                               int32_t weight_dtype, int32_t device, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* B200TRAIN_H_ */

@@ -1,4 +1,4 @@
-"""ctypes binding of ``libb200attn.so`` (the C ABI declared in ``include/b200attn.h`` and ``include/b200moe.h``).
+"""ctypes binding of ``libb200attn.so`` (the C ABI declared in ``include/b200attn.h``, ``include/b200moe.h`` and ``include/b200train.h``).
 
 There is deliberately no fallback: if the library cannot be loaded, or a call returns an
 error code, a ``RuntimeError`` is raised.
@@ -8,6 +8,8 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+
+import torch
 
 from . import build as _build
 
@@ -21,6 +23,8 @@ EXPORTS = (
     "b200moe_sizeof_gemm_params", "b200moe_grouped_gemm", "b200moe_gather_rows", "b200moe_combine_rows", "b200moe_row_dot",
     "b200moe_glu", "b200moe_glu_bwd", "b200moe_bias_grad", "b200moe_route",
 )
+TRAIN_EXPORTS = ("b200train_add_rms_norm", "b200train_norm_scratch_floats", "b200train_add_rms_norm_bwd")   # include/b200train.h
+TRAIN_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # B200TRAIN_BF16, _FP16, _FP32
 
 ROW_TILE = 128
 STATUS_WAIT_TIMEOUT = 1      # B200ATTN_STATUS_WAIT_TIMEOUT
@@ -123,6 +127,16 @@ def load() -> ctypes.CDLL:
             ("b200moe_glu_bwd", [vp, vp, vp, i64, i32, i32, vp]),
             ("b200moe_bias_grad", [vp, vp, vp, i32, i32, i32, vp]),
             ("b200moe_route", [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp]),
+        ):
+            fn = getattr(lib, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = args
+        f32 = ctypes.c_float
+        lib.b200train_norm_scratch_floats.restype = i64
+        lib.b200train_norm_scratch_floats.argtypes = [i64, i32, i32, i32]
+        for name, args in (
+            ("b200train_add_rms_norm", [vp, i64, vp, i64, vp, vp, vp, i64, i32, f32, i32, i32, i32, vp]),
+            ("b200train_add_rms_norm_bwd", [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, i32, f32, i32, i32, i32, vp]),
         ):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int

@@ -10,8 +10,8 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_PKG, "csrc")
 LIB_DIR = os.path.join(_PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libb200attn.so")
-HEADERS = [os.path.join(os.path.dirname(_PKG), "include", h) for h in ("b200attn.h", "b200moe.h")]
-UNITS = ("b200attn_api.cu", "b200moe_api.cu")   # one translation unit per header
+HEADERS = [os.path.join(os.path.dirname(_PKG), "include", h) for h in ("b200attn.h", "b200moe.h", "b200train.h")]
+UNITS = ("b200attn_api.cu", "b200moe_api.cu", "b200train_api.cu")   # one translation unit per header
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

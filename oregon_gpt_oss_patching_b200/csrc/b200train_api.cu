@@ -1,0 +1,185 @@
+// C ABI of the training-step entry points (declared in include/b200train.h): argument validation and kernel launches.
+// No device memory is allocated here and nothing synchronises.
+#include "../../include/b200train.h"
+
+#include <cuda_runtime.h>
+
+#include "host_common.cuh"
+#include "norm_kernels.cuh"
+
+namespace {
+
+using namespace b200train;
+using namespace b200attn::host;
+
+int sm_count(int device) {
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) return 148;
+  return n;
+}
+
+int elem_size(int dtype) { return dtype == B200TRAIN_FP32 ? 4 : 2; }
+bool known_dtype(int dtype) { return dtype >= B200TRAIN_BF16 && dtype <= B200TRAIN_FP32; }
+
+// ---------------------------------------------------------------- norm
+
+constexpr int kNormElems[] = {8, 16, 24, 32};   // elements a thread holds: the instances of the two kernels
+
+struct NormShape {
+  int elems = 0;     // one of kNormElems, 0: the row is too wide
+  int threads = 0;   // of a row lane
+  int lanes = 0;     // row lanes of a CTA
+  bool shift = false;
+};
+
+// Where there are rows for every SM several times over, a thread takes as much of a row as it can hold (fewer threads
+// meet at a row's barrier); where there are not, a row is spread over as many threads as it has 8-element pieces.
+NormShape norm_shape(long long rows, int cols, int dtype, int device, int cta_threads) {
+  NormShape s;
+  const int n = 16 / elem_size(dtype);
+  s.shift = cols % n != 0;
+  const int words = (cols + n - 1) / n + (s.shift ? 1 : 0);
+  const bool few = rows <= 2ll * sm_count(device);
+  for (int e : kNormElems) {
+    const int per_thread = e / n;
+    const int threads = ((words + per_thread - 1) / per_thread + 31) / 32 * 32;
+    if (threads > kNormMaxThreads) continue;
+    s.elems = e;
+    s.threads = threads;
+    if (few || threads == 32) break;
+  }
+  if (s.elems == 0) return s;
+  s.lanes = cta_threads / s.threads;
+  s.lanes = s.lanes < 1 ? 1 : (s.lanes > kNormMaxLanes ? kNormMaxLanes : s.lanes);
+  if (s.lanes > rows) s.lanes = rows < 1 ? 1 : (int)rows;
+  return s;
+}
+
+int norm_bwd_grid(const NormShape& s, long long rows, int device) {
+  const long long want = (rows + s.lanes - 1) / s.lanes, cap = sm_count(device);
+  const long long grid = want < cap ? want : cap;
+  return (int)((grid + 7) / 8 * 8);   // a lane's rows step by a multiple of 8 (see the kernel)
+}
+
+int check_norm_matrix(const void* p, int64_t stride, int64_t rows, int cols, int dtype) {
+  if (rows == 0) return B200ATTN_OK;   // (an empty tensor has no address)
+  if (p == nullptr) return B200ATTN_EINVAL;
+  const int n = 16 / elem_size(dtype);
+  if (!aligned16(p) || stride < 0) return B200ATTN_EALIGN;
+  if (cols % n == 0 ? stride % n != 0 : stride != cols) return B200ATTN_EALIGN;
+  return B200ATTN_OK;
+}
+
+int check_norm(int64_t rows, int cols, int dtype, int weight_dtype, const void* weight) {
+  if (rows < 0 || cols <= 0 || weight == nullptr || !known_dtype(dtype)) return B200ATTN_EINVAL;
+  if (weight_dtype != dtype && weight_dtype != B200TRAIN_FP32) return B200ATTN_EINVAL;
+  if (cols > B200TRAIN_NORM_MAX_COLS || rows > (1ll << 40) / cols) return B200ATTN_ESHAPE;
+  return aligned16(weight) ? B200ATTN_OK : B200ATTN_EALIGN;
+}
+
+// Calls f(T{}, W{}) with the element type and the weight type.
+template <typename F>
+int with_types(int dtype, int weight_dtype, F f) {
+  if (dtype == B200TRAIN_FP32) return f(float{}, float{});
+  if (dtype == B200TRAIN_BF16) return weight_dtype == B200TRAIN_FP32 ? f(__nv_bfloat16{}, float{}) : f(__nv_bfloat16{}, __nv_bfloat16{});
+  return weight_dtype == B200TRAIN_FP32 ? f(__half{}, float{}) : f(__half{}, __half{});
+}
+
+// Calls f(integral_constant<int, words a thread holds>, bool_constant<shift>).
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
+template <int N, typename F>
+int with_shape(const NormShape& s, F f) {
+  switch (s.elems) {
+    case 8: return s.shift ? f(Int<8 / N>{}, Int<1>{}) : f(Int<8 / N>{}, Int<0>{});
+    case 16: return s.shift ? f(Int<16 / N>{}, Int<1>{}) : f(Int<16 / N>{}, Int<0>{});
+    case 24: return s.shift ? f(Int<24 / N>{}, Int<1>{}) : f(Int<24 / N>{}, Int<0>{});
+    default: return s.shift ? f(Int<32 / N>{}, Int<1>{}) : f(Int<32 / N>{}, Int<0>{});
+  }
+}
+
+constexpr int kFwdThreads = 256, kBwdThreads = 512;
+
+}  // namespace
+
+extern "C" {
+
+int b200train_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                           const void* weight, void* y, void* h, int64_t rows, int32_t cols, float eps, int32_t dtype,
+                           int32_t weight_dtype, int32_t device, void* stream) {
+  int rc = check_norm(rows, cols, dtype, weight_dtype, weight);
+  if (rc) return rc;
+  if (rows > 0 && (residual == nullptr) != (h == nullptr)) return B200ATTN_EINVAL;
+  if ((rc = check_norm_matrix(x, x_stride, rows, cols, dtype)) || (rc = check_norm_matrix(y, cols, rows, cols, dtype))) return rc;
+  if (residual != nullptr &&
+      ((rc = check_norm_matrix(residual, residual_stride, rows, cols, dtype)) || (rc = check_norm_matrix(h, cols, rows, cols, dtype))))
+    return rc;
+  if ((rc = check_device(device))) return rc;
+  const NormShape s = norm_shape(rows, cols, dtype, device, kFwdThreads);
+  if (s.elems == 0) return B200ATTN_ESHAPE;
+  if (rows == 0) return B200ATTN_OK;
+  const long long grid = (rows + s.lanes - 1) / s.lanes;
+  if (grid > 0x7fffffffll) return B200ATTN_ESHAPE;
+  DeviceGuard guard(device);
+  if (!guard.ok) return B200ATTN_ECUDA;
+  return with_types(dtype, weight_dtype, [&](auto t, auto w) {
+    using T = decltype(t);
+    using W = decltype(w);
+    NormArgs<T, W> a{static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const W*>(weight), static_cast<T*>(y),
+                     static_cast<T*>(h), x_stride, residual_stride, rows, cols, eps};
+    return with_shape<Elem<T>::N>(s, [&](auto vpt, auto shift) {
+      add_rms_norm_kernel<T, W, decltype(vpt)::value, decltype(shift)::value != 0>
+          <<<(unsigned)grid, dim3(s.threads, s.lanes), 0, static_cast<cudaStream_t>(stream)>>>(a);
+      return launch_status();
+    });
+  });
+}
+
+int64_t b200train_norm_scratch_floats(int64_t rows, int32_t cols, int32_t dtype, int32_t device) {
+  if (rows <= 0 || cols <= 0 || cols > B200TRAIN_NORM_MAX_COLS || !known_dtype(dtype)) return 0;
+  const NormShape s = norm_shape(rows, cols, dtype, device, kBwdThreads);
+  return s.elems == 0 ? 0 : (int64_t)norm_bwd_grid(s, rows, device) * cols;
+}
+
+int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
+                               int64_t h_stride, const void* weight, void* dx, void* dweight, float* scratch,
+                               int64_t scratch_floats, int64_t rows, int32_t cols, float eps, int32_t dtype,
+                               int32_t weight_dtype, int32_t device, void* stream) {
+  int rc = check_norm(rows, cols, dtype, weight_dtype, weight);
+  if (rc) return rc;
+  if ((rc = check_norm_matrix(dy, dy_stride, rows, cols, dtype)) || (rc = check_norm_matrix(h, h_stride, rows, cols, dtype)) ||
+      (rc = check_norm_matrix(dx, cols, rows, cols, dtype)))
+    return rc;
+  if (dh != nullptr && (rc = check_norm_matrix(dh, dh_stride, rows, cols, dtype))) return rc;
+  if ((rc = check_device(device))) return rc;
+  const NormShape s = norm_shape(rows, cols, dtype, device, kBwdThreads);
+  if (s.elems == 0) return B200ATTN_ESHAPE;
+  DeviceGuard guard(device);
+  if (!guard.ok) return B200ATTN_ECUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0)
+    return dweight == nullptr || cudaMemsetAsync(dweight, 0, (size_t)cols * elem_size(weight_dtype), st) == cudaSuccess ? B200ATTN_OK
+                                                                                                                         : B200ATTN_ECUDA;
+  const int grid = norm_bwd_grid(s, rows, device);
+  if (dweight != nullptr && (scratch == nullptr || scratch_floats < (int64_t)grid * cols)) return B200ATTN_ESCRATCH;
+  return with_types(dtype, weight_dtype, [&](auto t, auto w) {
+    using T = decltype(t);
+    using W = decltype(w);
+    NormBwdArgs<T, W> a{static_cast<const T*>(dy), static_cast<const T*>(dh), static_cast<const T*>(h), static_cast<const W*>(weight),
+                        static_cast<T*>(dx), dweight != nullptr ? scratch : nullptr, dy_stride, dh_stride, h_stride, rows, cols, eps};
+    int rc2 = with_shape<Elem<T>::N>(s, [&](auto vpt, auto shift) {
+      constexpr auto kernel = add_rms_norm_bwd_kernel<T, W, decltype(vpt)::value, decltype(shift)::value != 0>;
+      const size_t smem = (size_t)s.lanes * cols * sizeof(float);
+      if (int e = set_smem<kernel>(kNormMaxThreads * 32 * sizeof(float))) return e;
+      kernel<<<grid, dim3(s.threads, s.lanes), smem, st>>>(a);
+      return launch_status();
+    });
+    if (rc2 || dweight == nullptr) return rc2;
+    norm_dw_kernel<W><<<(cols + 31) / 32, dim3(32, 32), 0, st>>>(scratch, static_cast<W*>(dweight), grid, cols);
+    return launch_status();
+  });
+}
+
+}  // extern "C"

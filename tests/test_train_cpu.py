@@ -1,0 +1,83 @@
+"""The training-step entry points without a GPU: the ABI is exported and refuses bad arguments, the Python side refuses bad tensors."""
+import os
+import re
+
+import pytest
+import torch
+
+from oregon_gpt_oss_patching_b200 import _cabi, build
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _cabi.load()
+
+
+def test_every_declared_symbol_is_exported(lib):
+    header = open(os.path.join(ROOT, "include", "b200train.h")).read()
+    header = re.sub(r"/\*.*?\*/", "", header, flags=re.S)
+    declared = set(re.findall(r"\b(b200train_[a-z_0-9]+)\s*\(", header))
+    assert declared == set(_cabi.TRAIN_EXPORTS)
+    for name in declared:
+        assert hasattr(lib, name), name
+    enum = dict(re.findall(r"(B200TRAIN_(?:BF16|FP16|FP32)) = (\d)", header))
+    assert {int(enum["B200TRAIN_BF16"]), int(enum["B200TRAIN_FP16"]), int(enum["B200TRAIN_FP32"])} == {0, 1, 2}
+    assert _cabi.TRAIN_DTYPES[torch.bfloat16] == int(enum["B200TRAIN_BF16"])
+    assert _cabi.TRAIN_DTYPES[torch.float16] == int(enum["B200TRAIN_FP16"])
+    assert _cabi.TRAIN_DTYPES[torch.float32] == int(enum["B200TRAIN_FP32"])
+
+
+def test_norm_arguments_are_validated(lib):
+    buf = torch.zeros(1 << 12, dtype=torch.float32)
+    p = buf.data_ptr()
+
+    def fwd(x=p, xs=64, r=None, rs=0, w=p, y=p, h=None, rows=2, cols=64, dtype=0, wdtype=0):
+        return lib.b200train_add_rms_norm(x, xs, r, rs, w, y, h, rows, cols, 1e-5, dtype, wdtype, 0, None)
+
+    assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(y=None) == -1
+    assert fwd(rows=-1) == -1 and fwd(cols=0) == -1
+    assert fwd(dtype=3) == -1 and fwd(dtype=-1) == -1 and fwd(dtype=0, wdtype=1) == -1 and fwd(dtype=2, wdtype=0) == -1
+    assert fwd(r=p, rs=64) == -1 and fwd(h=p) == -1                       # a residual and its sum come together
+    assert fwd(cols=16385, xs=16385) == -2
+    assert fwd(rows=1 << 40) == -2
+    assert fwd(x=p + 2) == -4 and fwd(w=p + 4) == -4 and fwd(xs=60) == -4 and fwd(xs=-64) == -4
+    assert fwd(cols=63, xs=64) == -4                                      # rows off the 16-byte grid must be contiguous
+    assert fwd(r=p, rs=65, h=p) == -4
+
+    def bwd(dy=p, dys=64, dh=None, h=p, w=p, dx=p, dw=None, rows=2, cols=64, dtype=0, wdtype=0):
+        return lib.b200train_add_rms_norm_bwd(dy, dys, dh, 64, h, 64, w, dx, dw, None, 0, rows, cols, 1e-5, dtype, wdtype, 0, None)
+
+    assert bwd(dy=None) == -1 and bwd(h=None) == -1 and bwd(dx=None) == -1 and bwd(w=None) == -1 and bwd(wdtype=1) == -1
+    assert bwd(dys=12) == -4 and bwd(dh=p + 2) == -4 and bwd(cols=20000) == -2
+    assert lib.b200train_norm_scratch_floats(0, 64, 0, 0) == 0
+    assert lib.b200train_norm_scratch_floats(4, 64, 7, 0) == 0
+    assert lib.b200train_norm_scratch_floats(10, 64, 0, 0) >= 64
+    if not torch.cuda.is_available():
+        assert fwd() in (-5, -6) and bwd() in (-5, -6)                    # no sm_100 device
+
+
+def test_norm_refuses_bad_tensors():
+    from oregon_gpt_oss_patching_b200.rms_norm import add_rms_norm, rms_norm
+    x = torch.zeros(3, 8)
+    with pytest.raises(RuntimeError, match="needs CUDA tensors"):
+        rms_norm(x, torch.ones(8))
+    with pytest.raises(RuntimeError, match="needs CUDA tensors"):
+        add_rms_norm(x, x, torch.ones(8))
+    if not torch.cuda.is_available():
+        return
+    x = x.cuda()
+    w = torch.ones(8, device="cuda")
+    for bad in (lambda: rms_norm(x.double(), w), lambda: rms_norm(x, w.half()), lambda: rms_norm(x.int(), w)):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: rms_norm(x, w[:7]), lambda: add_rms_norm(x, x[:2], w), lambda: add_rms_norm(x, x.half(), w),
+                lambda: rms_norm(x, w, -1.0), lambda: rms_norm(x, w, float("nan")), lambda: rms_norm(x.sum(), w)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        rms_norm(x, w.cpu())
+    with pytest.raises(RuntimeError, match="code -2"):
+        rms_norm(torch.zeros(2, 16392, device="cuda"), torch.ones(16392, device="cuda"))
