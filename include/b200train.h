@@ -25,6 +25,8 @@ extern "C" {
 /* Element types. */
 enum { B200TRAIN_BF16 = 0, B200TRAIN_FP16 = 1, B200TRAIN_FP32 = 2 };
 
+enum { B200TRAIN_EOVERLAP = -10 }; /* two tensors of one call, one of which is written, share memory */
+
 #define B200TRAIN_NORM_MAX_COLS 16384 /* widest row of the norm */
 
 /*
@@ -56,6 +58,30 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
                                int64_t h_stride, const void* weight, void* dx, void* dweight, float* scratch,
                                int64_t scratch_floats, int64_t rows, int32_t cols, float eps, int32_t dtype,
                                int32_t weight_dtype, int32_t device, void* stream);
+
+/*
+ * The global norm of many tensors, clipping by it, and the SGD update with the clip folded in.
+ *   grads, params, counts, dtypes   HOST arrays of `tensors` entries, read during the call: device addresses (element
+ *                                   aligned), elements (>= 0), element types.  A tensor's elements are contiguous; no two
+ *                                   tensors of a call that writes may overlap (B200TRAIN_EOVERLAP).
+ *   scratch                         device fp64, b200train_clip_scratch_doubles(...) of them
+ *   norm                            out, device fp32: n = sqrt(sum of g^2 over all tensors).  Squares are fp32, sums beyond a
+ *                                   few hundred of them fp64: an element above 1.8e19 makes n infinite.
+ * c = min(1, max_norm / (n + 1e-6)), max_norm >= 0; a NaN norm makes c NaN, an infinite one 0.  No value is read by the host.
+ */
+int64_t b200train_clip_scratch_doubles(int64_t tensors, int32_t device);
+
+/* norm only. */
+int b200train_grad_norm(const int64_t* grads, const int64_t* counts, const int32_t* dtypes, int64_t tensors, double* scratch,
+                        int64_t scratch_doubles, float* norm, int32_t device, void* stream);
+
+/* g <- round(c * g); nothing is written where c = 1.  torch.nn.utils.clip_grad_norm_ as one pass each way. */
+int b200train_clip_grads(const int64_t* grads, const int64_t* counts, const int32_t* dtypes, int64_t tensors, float max_norm,
+                         double* scratch, int64_t scratch_doubles, float* norm, int32_t device, void* stream);
+
+/* p <- round(p - lr * c * g), rounded once; the gradients are left as they are.  A parameter has its gradient's type. */
+int b200train_clipped_sgd(const int64_t* grads, const int64_t* params, const int64_t* counts, const int32_t* dtypes, int64_t tensors,
+                          float lr, float max_norm, double* scratch, int64_t scratch_doubles, float* norm, int32_t device, void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,3 +23,12 @@ def add_rms_norm_bwd(h, weight, dy, dh, eps):
     if dh is not None:
         dx = dx + dh.double()
     return dx, (dy * n).reshape(-1, h.shape[-1]).sum(0)
+
+
+def grad_norm(grads):
+    return torch.sqrt(sum((g.double() ** 2).sum() for g in grads))
+
+
+def clip_coefficient(norm, max_norm):
+    """min(1, max_norm / (norm + 1e-6)), NaN for a NaN norm: ``torch.nn.utils.clip_grad_norm_``."""
+    return torch.clamp(max_norm / (norm + 1e-6), max=1.0)

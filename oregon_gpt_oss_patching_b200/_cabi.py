@@ -23,7 +23,10 @@ EXPORTS = (
     "b200moe_sizeof_gemm_params", "b200moe_grouped_gemm", "b200moe_gather_rows", "b200moe_combine_rows", "b200moe_row_dot",
     "b200moe_glu", "b200moe_glu_bwd", "b200moe_bias_grad", "b200moe_route",
 )
-TRAIN_EXPORTS = ("b200train_add_rms_norm", "b200train_norm_scratch_floats", "b200train_add_rms_norm_bwd")   # include/b200train.h
+TRAIN_EXPORTS = (            # include/b200train.h
+    "b200train_add_rms_norm", "b200train_norm_scratch_floats", "b200train_add_rms_norm_bwd", "b200train_clip_scratch_doubles",
+    "b200train_grad_norm", "b200train_clip_grads", "b200train_clipped_sgd",
+)
 TRAIN_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # B200TRAIN_BF16, _FP16, _FP32
 
 ROW_TILE = 128
@@ -134,7 +137,12 @@ def load() -> ctypes.CDLL:
         f32 = ctypes.c_float
         lib.b200train_norm_scratch_floats.restype = i64
         lib.b200train_norm_scratch_floats.argtypes = [i64, i32, i32, i32]
+        lib.b200train_clip_scratch_doubles.restype = i64
+        lib.b200train_clip_scratch_doubles.argtypes = [i64, i32]
         for name, args in (
+            ("b200train_grad_norm", [vp, vp, vp, i64, vp, i64, vp, i32, vp]),
+            ("b200train_clip_grads", [vp, vp, vp, i64, f32, vp, i64, vp, i32, vp]),
+            ("b200train_clipped_sgd", [vp, vp, vp, vp, i64, f32, f32, vp, i64, vp, i32, vp]),
             ("b200train_add_rms_norm", [vp, i64, vp, i64, vp, vp, vp, i64, i32, f32, i32, i32, i32, vp]),
             ("b200train_add_rms_norm_bwd", [vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, i32, f32, i32, i32, i32, vp]),
         ):

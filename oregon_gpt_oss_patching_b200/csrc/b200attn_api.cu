@@ -1,6 +1,7 @@
 // C ABI of the library (declared in include/b200attn.h): argument validation, TMA tensor
 // maps, kernel launches.  No device memory is allocated here and nothing synchronises.
 #include "../../include/b200attn.h"
+#include "../../include/b200train.h"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -144,6 +145,7 @@ const char* b200attn_strerror(int code) {
     case B200ATTN_ETENSORMAP: return "the driver rejected a TMA tensor map";
     case B200ATTN_ESCRATCH: return "scratch buffer missing";
     case B200ATTN_ETOOLARGE: return "problem exceeds the fixed scratch of b200attn_bwd_static_scratch (B*Hq*S_pad > B200ATTN_STATIC_MAX_ROWS)";
+    case B200TRAIN_EOVERLAP: return "two tensors of one call share memory, and one of them is written";
     default: return "unknown b200attn error code";
   }
 }

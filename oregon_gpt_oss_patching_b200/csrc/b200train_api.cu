@@ -4,6 +4,12 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <memory>
+#include <new>
+#include <utility>
+
+#include "clip_kernels.cuh"
 #include "host_common.cuh"
 #include "norm_kernels.cuh"
 
@@ -102,6 +108,110 @@ int with_shape(const NormShape& s, F f) {
 
 constexpr int kFwdThreads = 256, kBwdThreads = 512;
 
+// ---------------------------------------------------------------- clip
+
+constexpr int kClipCtasPerSm = 8;
+
+int clip_grid(int device) { return sm_count(device) * kClipCtasPerSm; }
+
+enum class ClipOp { kNorm, kClip, kSgd };
+
+// Fills a table with the tensors [begin, begin + kClipTensors), empty ones left out, and returns how many were looked at.
+int64_t fill_table(ClipTable* t, const int64_t* grads, const int64_t* params, const int64_t* counts, const int32_t* dtypes, int64_t begin,
+                   int64_t tensors) {
+  t->tensors = 0;
+  unsigned chunks = 0;
+  int64_t i = begin;
+  for (; i < tensors && t->tensors < kClipTensors; ++i) {
+    if (counts[i] == 0) continue;
+    const long long n = 16 / elem_size(dtypes[i]);
+    const long long off = (long long)(((uint64_t)grads[i] & 15u) / elem_size(dtypes[i]));
+    const int k = t->tensors++;
+    t->grad[k] = reinterpret_cast<void*>((uintptr_t)grads[i]);
+    t->param[k] = params != nullptr ? reinterpret_cast<void*>((uintptr_t)params[i]) : nullptr;
+    t->count[k] = counts[i];
+    t->first[k] = chunks;
+    t->dtype[k] = (unsigned char)dtypes[i];
+    chunks += (unsigned)(((off + counts[i] + n - 1) / n + kChunkWords - 1) / kChunkWords);
+  }
+  t->chunks = chunks;
+  return i - begin;
+}
+
+// Whether any two of the tensors that are written share memory, with one another or with a tensor that is read.
+bool overlaps(const int64_t* a, const int64_t* b, const int64_t* counts, const int32_t* dtypes, int64_t n) {
+  std::pair<uint64_t, uint64_t> few[128];
+  std::unique_ptr<std::pair<uint64_t, uint64_t>[]> many;
+  const int64_t all = b != nullptr ? 2 * n : n;
+  auto* s = few;
+  if (all > 128) {
+    many.reset(new (std::nothrow) std::pair<uint64_t, uint64_t>[all]);
+    if (!many) return true;
+    s = many.get();
+  }
+  int64_t k = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    if (counts[i] == 0) continue;
+    const uint64_t bytes = (uint64_t)counts[i] * elem_size(dtypes[i]);
+    s[k++] = {(uint64_t)a[i], (uint64_t)a[i] + bytes};
+    if (b != nullptr) s[k++] = {(uint64_t)b[i], (uint64_t)b[i] + bytes};
+  }
+  std::sort(s, s + k);
+  for (int64_t i = 1; i < k; ++i)
+    if (s[i].first < s[i - 1].second) return true;
+  return false;
+}
+
+int run_clip(ClipOp op, const int64_t* grads, const int64_t* params, const int64_t* counts, const int32_t* dtypes, int64_t tensors, float lr,
+             float max_norm, double* scratch, int64_t scratch_doubles, float* norm, int device, void* stream) {
+  if (tensors < 0 || norm == nullptr || (tensors > 0 && (grads == nullptr || counts == nullptr || dtypes == nullptr))) return B200ATTN_EINVAL;
+  if (op == ClipOp::kSgd && tensors > 0 && params == nullptr) return B200ATTN_EINVAL;
+  if (op != ClipOp::kNorm && !(max_norm >= 0.f)) return B200ATTN_EINVAL;
+  if (tensors > (1 << 24)) return B200ATTN_ESHAPE;
+  int64_t left = 1ll << 43;   // elements in all: at most 2^30 chunks, and one more a tensor, fit the 32 bits of a chunk's number
+  for (int64_t i = 0; i < tensors; ++i) {
+    if (!known_dtype(dtypes[i]) || counts[i] < 0) return B200ATTN_EINVAL;
+    if (counts[i] > left) return B200ATTN_ESHAPE;
+    left -= counts[i];
+    if (counts[i] == 0) continue;
+    const int64_t size = elem_size(dtypes[i]);
+    if (grads[i] == 0 || (op == ClipOp::kSgd && params[i] == 0)) return B200ATTN_EINVAL;
+    if (grads[i] % size != 0 || (op == ClipOp::kSgd && params[i] % size != 0)) return B200ATTN_EALIGN;
+  }
+  if (op != ClipOp::kNorm && overlaps(grads, op == ClipOp::kSgd ? params : nullptr, counts, dtypes, tensors)) return B200TRAIN_EOVERLAP;
+  int rc = check_device(device);
+  if (rc) return rc;
+  if (scratch == nullptr || scratch_doubles < b200train_clip_scratch_doubles(tensors, device)) return B200ATTN_ESCRATCH;
+  DeviceGuard guard(device);
+  if (!guard.ok) return B200ATTN_ECUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int cap = clip_grid(device);
+  ClipTable t;
+  int parts = 0;
+  for (int64_t i = 0; i < tensors;) {
+    i += fill_table(&t, grads, params, counts, dtypes, i, tensors);
+    if (t.tensors == 0) continue;
+    const int grid = t.chunks < (unsigned)cap ? (int)t.chunks : cap;
+    grad_sumsq_kernel<<<grid, kClipThreads, 0, st>>>(t, scratch + parts);
+    parts += grid;
+    if ((rc = launch_status())) return rc;
+  }
+  if (op == ClipOp::kNorm || parts == 0) {
+    grad_norm_kernel<<<1, kClipThreads, 0, st>>>(scratch, parts, norm);
+    return launch_status();
+  }
+  for (int64_t i = 0; i < tensors;) {
+    if (tensors > kClipTensors) i += fill_table(&t, grads, params, counts, dtypes, i, tensors);
+    else i = tensors;   // (the table of the first kernel serves again)
+    if (t.tensors == 0) continue;
+    const int grid = t.chunks < (unsigned)cap ? (int)t.chunks : cap;
+    if (op == ClipOp::kSgd) clip_apply_kernel<true><<<grid, kClipThreads, 0, st>>>(t, scratch, parts, max_norm, lr, norm);
+    else clip_apply_kernel<false><<<grid, kClipThreads, 0, st>>>(t, scratch, parts, max_norm, 0.f, norm);
+    if ((rc = launch_status())) return rc;
+  }
+  return B200ATTN_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -180,6 +290,27 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
     norm_dw_kernel<W><<<(cols + 31) / 32, dim3(32, 32), 0, st>>>(scratch, static_cast<W*>(dweight), grid, cols);
     return launch_status();
   });
+}
+
+// (one partial a CTA of every launch; every launch but the last takes kClipTensors tensors)
+int64_t b200train_clip_scratch_doubles(int64_t tensors, int32_t device) {
+  if (tensors < 0) return 0;
+  return (tensors / kClipTensors + 1) * clip_grid(device);
+}
+
+int b200train_grad_norm(const int64_t* grads, const int64_t* counts, const int32_t* dtypes, int64_t tensors, double* scratch,
+                        int64_t scratch_doubles, float* norm, int32_t device, void* stream) {
+  return run_clip(ClipOp::kNorm, grads, nullptr, counts, dtypes, tensors, 0.f, 0.f, scratch, scratch_doubles, norm, device, stream);
+}
+
+int b200train_clip_grads(const int64_t* grads, const int64_t* counts, const int32_t* dtypes, int64_t tensors, float max_norm,
+                         double* scratch, int64_t scratch_doubles, float* norm, int32_t device, void* stream) {
+  return run_clip(ClipOp::kClip, grads, nullptr, counts, dtypes, tensors, 0.f, max_norm, scratch, scratch_doubles, norm, device, stream);
+}
+
+int b200train_clipped_sgd(const int64_t* grads, const int64_t* params, const int64_t* counts, const int32_t* dtypes, int64_t tensors,
+                          float lr, float max_norm, double* scratch, int64_t scratch_doubles, float* norm, int32_t device, void* stream) {
+  return run_clip(ClipOp::kSgd, grads, params, counts, dtypes, tensors, lr, max_norm, scratch, scratch_doubles, norm, device, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,180 @@
+// The global norm of many gradients, clipping by it, and the state-free SGD update with the clip folded in.
+//
+//   n = sqrt(sum over all tensors of g^2),  c = min(1, max_norm / (n + 1e-6)),  g <- round(c g)   or   p <- round(p - lr c g)
+//
+// Two launches: `grad_sumsq_kernel` reads every gradient once and leaves one partial sum a CTA; each CTA of the second
+// kernel adds the same partials in the same order, so all of them hold the same c without a third launch, a counter or
+// atomics, and writes back (nothing, where c = 1).  Both are bound by HBM: clipping cannot do without reading the gradients
+// twice (unless they fit in L2) and writing them once; the folded update reads gradients twice and parameters once and
+// writes the parameters, where clipping first and updating then moves half as much again.
+//
+// The tensors' addresses and sizes travel as a kernel parameter (no copy to the device, nothing to keep alive, nothing for a
+// captured graph to find changed).  Work is cut into chunks of kChunkWords 16-byte words of the 16-byte grid that covers a
+// tensor; a word at a tensor's end that it shares with other memory is moved element by element.
+#pragma once
+#include "elem_types.cuh"
+
+namespace b200train {
+
+constexpr int kClipThreads = 256;
+constexpr int kClipTensors = 256;     // of one launch
+constexpr int kChunkWords = 2048;     // 32 KB
+
+struct ClipTable {
+  void* grad[kClipTensors];
+  void* param[kClipTensors];
+  long long count[kClipTensors];      // elements
+  unsigned first[kClipTensors];       // a tensor's first chunk
+  unsigned char dtype[kClipTensors];
+  int tensors;
+  unsigned chunks;
+};
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The sum over the CTA, in every thread.
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[kClipThreads / 32];
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_sum((threadIdx.x & 31) < kClipThreads / 32 ? part[threadIdx.x & 31] : 0.0);
+}
+
+// The tensor that holds a chunk: the last one whose first chunk is not behind it.
+__device__ __forceinline__ int tensor_of(const ClipTable& t, unsigned chunk) {
+  int lo = 0, hi = t.tensors - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= chunk) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// A chunk of one tensor: words [begin, end) of the 16-byte grid, the tensor's elements being [off, off + count) of that grid.
+template <typename T>
+struct Chunk {
+  static constexpr int N = Elem<T>::N;
+  long long begin, end, off, last;   // last = off + count
+  __device__ __forceinline__ Chunk(const void* grad, long long count, unsigned index) {
+    off = (long long)((reinterpret_cast<uintptr_t>(grad) & 15u) / sizeof(T));
+    last = off + count;
+    const long long words = (last + N - 1) / N;
+    begin = (long long)index * kChunkWords;
+    end = begin + kChunkWords < words ? begin + kChunkWords : words;
+  }
+  __device__ __forceinline__ bool inside(long long w) const { return w * N >= off && (w + 1) * N <= last; }
+  // element e of word w relative to the tensor's first element, and whether the tensor has it
+  __device__ __forceinline__ long long at(long long w, int e) const { return w * N + e - off; }
+  __device__ __forceinline__ bool has(long long w, int e) const { return w * N + e >= off && w * N + e < last; }
+  __device__ __forceinline__ void load(const T* p, long long w, bool vector, float* f) const {
+    if (vector && inside(w)) {
+      unpack<T>(*reinterpret_cast<const uint4*>(p + at(w, 0)), f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = has(w, e) ? Elem<T>::load1(p + at(w, e)) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(T* p, long long w, bool vector, const float* f) const {
+    if (vector && inside(w)) {
+      *reinterpret_cast<uint4*>(p + at(w, 0)) = pack<T>(f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (has(w, e)) Elem<T>::store1(p + at(w, e), f[e]);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float chunk_sumsq(const void* grad, long long count, unsigned index) {
+  const Chunk<T> c(grad, count, index);
+  const T* g = static_cast<const T*>(grad);
+  float sum = 0.f;
+#pragma unroll 4
+  for (long long w = c.begin + threadIdx.x; w < c.end; w += kClipThreads) {
+    float f[Elem<T>::N];
+    c.load(g, w, true, f);
+#pragma unroll
+    for (int e = 0; e < Elem<T>::N; ++e) sum = fmaf(f[e], f[e], sum);
+  }
+  return sum;
+}
+
+// A thread's sum over a chunk is fp32 (a few hundred terms), everything above it fp64.
+__global__ void __launch_bounds__(kClipThreads) grad_sumsq_kernel(const __grid_constant__ ClipTable t, double* partials) {
+  double sum = 0.0;
+  for (unsigned chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+    const int i = tensor_of(t, chunk);
+    const unsigned index = chunk - t.first[i];
+    float s;
+    if (t.dtype[i] == 0) s = chunk_sumsq<__nv_bfloat16>(t.grad[i], t.count[i], index);
+    else if (t.dtype[i] == 1) s = chunk_sumsq<__half>(t.grad[i], t.count[i], index);
+    else s = chunk_sumsq<float>(t.grad[i], t.count[i], index);
+    sum += (double)s;
+  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+}
+
+template <typename T, bool kUpdate>
+__device__ __forceinline__ void chunk_apply(void* grad, void* param, long long count, unsigned index, float scale) {
+  const Chunk<T> c(grad, count, index);
+  T* g = static_cast<T*>(grad);
+  T* p = static_cast<T*>(param);
+  // a parameter that lies otherwise on the 16-byte grid than its gradient is moved element by element
+  const bool same = !kUpdate || ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(param)) & 15u) == 0;
+#pragma unroll 4
+  for (long long w = c.begin + threadIdx.x; w < c.end; w += kClipThreads) {
+    float f[Elem<T>::N], q[Elem<T>::N];
+    c.load(g, w, true, f);
+    if (kUpdate) {
+      c.load(p, w, same, q);
+#pragma unroll
+      for (int e = 0; e < Elem<T>::N; ++e) q[e] = fmaf(-scale, f[e], q[e]);
+      c.store(p, w, same, q);
+    } else {
+#pragma unroll
+      for (int e = 0; e < Elem<T>::N; ++e) f[e] *= scale;
+      c.store(g, w, true, f);
+    }
+  }
+}
+
+// kUpdate: p <- p - lr c g, otherwise g <- c g.  `norm` gets sqrt of the sum of the partials.
+template <bool kUpdate>
+__global__ void __launch_bounds__(kClipThreads)
+clip_apply_kernel(const __grid_constant__ ClipTable t, const double* __restrict__ partials, int parts, float max_norm, float lr,
+                  float* __restrict__ norm) {
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kClipThreads) sum += partials[i];
+  const float n = (float)sqrt(block_sum(sum));
+  if (blockIdx.x == 0 && threadIdx.x == 0 && norm != nullptr) *norm = n;
+  float scale = max_norm / (n + 1e-6f);
+  if (scale >= 1.f) {   // (not where it is NaN: that goes into the gradients)
+    if (!kUpdate) return;
+    scale = 1.f;
+  }
+  if (kUpdate) scale *= lr;
+  for (unsigned chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+    const int i = tensor_of(t, chunk);
+    const unsigned index = chunk - t.first[i];
+    if (t.dtype[i] == 0) chunk_apply<__nv_bfloat16, kUpdate>(t.grad[i], t.param[i], t.count[i], index, scale);
+    else if (t.dtype[i] == 1) chunk_apply<__half, kUpdate>(t.grad[i], t.param[i], t.count[i], index, scale);
+    else chunk_apply<float, kUpdate>(t.grad[i], t.param[i], t.count[i], index, scale);
+  }
+}
+
+// norm <- sqrt of the sum of the partials (the norm alone is asked for).
+__global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const double* __restrict__ partials, int parts, float* __restrict__ norm) {
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kClipThreads) sum += partials[i];
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) *norm = (float)sqrt(sum);
+}
+
+}  // namespace b200train

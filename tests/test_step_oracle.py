@@ -38,3 +38,17 @@ def test_norm_restates_the_installed_module():
     # the module computes in fp32: a sum of 24 squares, a root, two products
     assert torch.allclose(mod(x).double(), y, rtol=32 * 2.0 ** -24, atol=0)
     assert torch.equal(h, x.double())
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 0.7, 100.0, float("inf")])
+def test_clip_restates_torch(max_norm):
+    g = torch.Generator().manual_seed(3)
+    params = [torch.nn.Parameter(torch.zeros(n, dtype=torch.float64)) for n in (1, 5, 30)]
+    for p in params:
+        p.grad = torch.randn(p.shape, generator=g, dtype=torch.float64)
+    before = [p.grad.clone() for p in params]
+    norm = torch.nn.utils.clip_grad_norm_(params, max_norm)
+    assert torch.allclose(norm, step_fp64.grad_norm(before), rtol=1e-14)
+    c = step_fp64.clip_coefficient(norm, max_norm)
+    for p, b in zip(params, before):
+        assert torch.allclose(p.grad, b * c, rtol=1e-14)

@@ -81,3 +81,62 @@ def test_norm_refuses_bad_tensors():
         rms_norm(x, w.cpu())
     with pytest.raises(RuntimeError, match="code -2"):
         rms_norm(torch.zeros(2, 16392, device="cuda"), torch.ones(16392, device="cuda"))
+
+
+def test_clip_arguments_are_validated(lib):
+    import array
+    import ctypes
+    buf = torch.zeros(1 << 8, dtype=torch.float32)
+    p = buf.data_ptr()
+    norm = ctypes.c_float(7.0)
+
+    def call(kind="clip", grads=(p,), params=(p + 512,), counts=(16,), dtypes=(2,), max_norm=1.0, scratch=p, doubles=1 << 30, out=None, n=None):
+        keep = [array.array(c, v) for c, v in (("q", grads), ("q", params), ("q", counts), ("i", dtypes))]
+        host = [a.buffer_info()[0] for a in keep]
+        n = len(grads) if n is None else n
+        out = ctypes.addressof(norm) if out is None else out
+        tail = (scratch, doubles, out, 0, None)
+        if kind == "norm":
+            return lib.b200train_grad_norm(host[0], host[2], host[3], n, *tail)
+        if kind == "clip":
+            return lib.b200train_clip_grads(host[0], host[2], host[3], n, max_norm, *tail)
+        return lib.b200train_clipped_sgd(host[0], host[1], host[2], host[3], n, 0.1, max_norm, *tail)
+
+    for kind in ("norm", "clip", "sgd"):
+        assert call(kind, out=0) == -1 and call(kind, n=-1) == -1
+        assert call(kind, dtypes=(3,)) == -1 and call(kind, dtypes=(-1,)) == -1 and call(kind, counts=(-1,)) == -1
+        assert call(kind, grads=(0,)) == -1 and call(kind, grads=(p + 2,)) == -4
+        assert call(kind, counts=(1 << 44,)) == -2
+        assert call(kind, grads=(p, p + 1024), params=(p + 2048, p + 4096), counts=(1 << 42, (1 << 42) + 1), dtypes=(2, 2)) == -2
+        if not torch.cuda.is_available():
+            assert call(kind) in (-5, -6)
+    for kind in ("clip", "sgd"):
+        assert call(kind, max_norm=-1.0) == -1 and call(kind, max_norm=float("nan")) == -1
+        assert call(kind, grads=(p, p + 60), params=(p + 512, p + 640), counts=(16, 16), dtypes=(2, 2)) == -10
+    assert call("sgd", params=(0,)) == -1 and call("sgd", params=(p + 513,)) == -4
+    assert call("sgd", params=(p + 32,)) == -10                            # a parameter on its own gradient
+    assert lib.b200train_clip_scratch_doubles(-1, 0) == 0
+    assert lib.b200train_clip_scratch_doubles(257, 0) == 2 * lib.b200train_clip_scratch_doubles(0, 0)
+    assert "share memory" in _cabi.strerror(-10)
+
+
+def test_clip_refuses_bad_tensors():
+    from oregon_gpt_oss_patching_b200.grad_clip import clip_grad_norm, clipped_sgd_step, global_grad_norm
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.zeros(4)
+    for call in (lambda: clip_grad_norm([p], 1.0), lambda: clipped_sgd_step([p], 0.1, 1.0), lambda: global_grad_norm([p])):
+        with pytest.raises(RuntimeError, match="needs CUDA tensors"):
+            call()
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            clip_grad_norm([p], bad)
+        with pytest.raises(ValueError, match="max_norm"):
+            clipped_sgd_step([p], 0.1, bad)
+    if not torch.cuda.is_available():
+        return
+    q = torch.nn.Parameter(torch.zeros(4, device="cuda", dtype=torch.float64))
+    q.grad = torch.zeros_like(q)
+    with pytest.raises(TypeError):
+        clip_grad_norm([q], 1.0)
+    with pytest.raises(RuntimeError):
+        global_grad_norm([p, q])
