@@ -90,6 +90,38 @@ int b200moe_grouped_gemm(const b200moe_gemm_params* p);
 int b200moe_route(const int64_t* indices, const float* weights, int32_t tokens, int32_t top_k, int32_t num_groups, int32_t rows,
                   int32_t* offsets, int32_t* row_token, int32_t* pos, float* row_weight, int32_t device, void* stream);
 
+/* Element types of the router's tensors. */
+enum { B200MOE_BF16 = 0, B200MOE_FP16 = 1, B200MOE_FP32 = 2 };
+
+#define B200MOE_ROUTER_MAX_EXPERTS 256
+#define B200MOE_ROUTER_MAX_TOP_K 32
+#define B200MOE_ROUTER_MAX_GROUPS 32
+
+/*
+ * The choice of experts, one launch.  Replaces the top-k and the softmax of GptOssTopKRouter.forward
+ * (modeling_gpt_oss.py:126-133: sigmoid 0, renormalize 1, scale 1, no bias, one group).
+ *   s = softmax(logits) over the experts, or sigmoid(logits);  v = s + bias, but -inf where the logit is (a masked expert)
+ *   with groups > 1 the experts form that many equal runs, a run's value is the sum of its two largest v that are not
+ *   -inf, and only the experts of the top_groups largest runs are eligible
+ *   indices[t,:] = the top_k largest v of the eligible, in falling order; ties, here and between runs, go to the lowest
+ *   index; NaN ranks above everything.  The order is that of the real numbers (fp64 where fp32 cannot tell two apart).
+ *   weights[t,j] = scale * s / (renormalize ? sum of the chosen s : 1), of the chosen; 0 where that sum is 0
+ *   logits    (tokens x experts) of `dtype`, `stride` elements from row to row;  bias: device fp32 (experts) or NULL
+ *   weights   out, (tokens x top_k) of `dtype`;  indices: out, device int64 (tokens x top_k)
+ * 1 <= top_k <= min(32, top_groups * experts / groups), experts <= 256, groups <= 32 divides experts.
+ */
+int b200moe_router_topk(const void* logits, int64_t stride, const float* bias, void* weights, int64_t* indices, int32_t tokens,
+                        int32_t experts, int32_t top_k, int32_t groups, int32_t top_groups, int32_t sigmoid, int32_t renormalize,
+                        float scale, int32_t dtype, int32_t device, void* stream);
+
+/*
+ * dlogits (tokens x experts, contiguous, fully overwritten) from dweights (tokens x top_k, contiguous) and the choice that
+ * b200moe_router_topk made; the scores are taken from the logits again.  The choice itself, and so the bias, has no gradient.
+ */
+int b200moe_router_topk_bwd(const void* logits, int64_t stride, const int64_t* indices, const void* dweights, void* dlogits, int32_t tokens,
+                            int32_t experts, int32_t top_k, int32_t sigmoid, int32_t renormalize, float scale, int32_t dtype, int32_t device,
+                            void* stream);
+
 /*
  * out[r,:] = src[row_src[r],:] * (row_scale ? row_scale[r] : 1) for row_src[r] >= 0, zeros for
  * row_src[r] < 0 (padding rows).  Replaces `hidden_states[token_idx]` (modeling_gpt_oss.py:104);

@@ -21,7 +21,8 @@ EXPORTS = (
     "b200attn_bwd_dq", "b200attn_bwd_dq_is_fused", "b200attn_bwd_static_scratch", "b200attn_umma_selftest",
     "b200attn_wait_selftest", "b200attn_rope",
     "b200moe_sizeof_gemm_params", "b200moe_grouped_gemm", "b200moe_gather_rows", "b200moe_combine_rows", "b200moe_row_dot",
-    "b200moe_glu", "b200moe_glu_bwd", "b200moe_bias_grad", "b200moe_route",
+    "b200moe_glu", "b200moe_glu_bwd", "b200moe_bias_grad", "b200moe_route", "b200moe_router_topk",
+    "b200moe_router_topk_bwd",
 )
 TRAIN_EXPORTS = (            # include/b200train.h
     "b200train_add_rms_norm", "b200train_norm_scratch_floats", "b200train_add_rms_norm_bwd", "b200train_clip_scratch_doubles",
@@ -54,6 +55,8 @@ class Params(ctypes.Structure):
 
 
 MOE_ROW_ALIGN = 128          # B200MOE_ROW_ALIGN
+MOE_ROUTER_MAX_EXPERTS, MOE_ROUTER_MAX_TOP_K, MOE_ROUTER_MAX_GROUPS = 256, 32, 32   # B200MOE_ROUTER_MAX_*
+MOE_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # B200MOE_BF16, _FP16, _FP32
 MOE_ROWS_NN, MOE_ROWS_NT, MOE_INNER_TN = 0, 1, 2
 
 
@@ -113,7 +116,7 @@ def load() -> ctypes.CDLL:
                                                ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
         lib.b200attn_wait_selftest.restype = ctypes.c_int
         lib.b200attn_wait_selftest.argtypes = [ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
-        vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+        vp, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
         lib.b200attn_rope.restype = ctypes.c_int
         lib.b200attn_rope.argtypes = [ctypes.POINTER(Tensor4), ctypes.POINTER(Tensor4), vp, vp, i64, i64, i32, i32, i32, i32, i32, vp]
         lib.b200moe_sizeof_gemm_params.restype = ctypes.c_size_t
@@ -130,11 +133,12 @@ def load() -> ctypes.CDLL:
             ("b200moe_glu_bwd", [vp, vp, vp, i64, i32, i32, vp]),
             ("b200moe_bias_grad", [vp, vp, vp, i32, i32, i32, vp]),
             ("b200moe_route", [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp]),
+            ("b200moe_router_topk", [vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, i32, i32, vp]),
+            ("b200moe_router_topk_bwd", [vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, f32, i32, i32, vp]),
         ):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
             fn.argtypes = args
-        f32 = ctypes.c_float
         lib.b200train_norm_scratch_floats.restype = i64
         lib.b200train_norm_scratch_floats.argtypes = [i64, i32, i32, i32]
         lib.b200train_clip_scratch_doubles.restype = i64

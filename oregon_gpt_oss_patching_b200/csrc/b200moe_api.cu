@@ -7,6 +7,7 @@
 
 #include "host_common.cuh"
 #include "moe_gemm_kernel.cuh"   // (includes moe_aux_kernels.cuh)
+#include "router_kernels.cuh"
 
 namespace {
 
@@ -55,6 +56,39 @@ int check_matrix(const void* p, int64_t cols) {
   if (p == nullptr) return B200ATTN_EINVAL;
   if (!aligned16(p) || cols % 8 != 0) return B200ATTN_EALIGN;
   return B200ATTN_OK;
+}
+
+int check_router(const void* logits, int64_t stride, int tokens, int experts, int top_k, int dtype) {
+  if (tokens < 0 || experts <= 0 || top_k <= 0 || dtype < B200MOE_BF16 || dtype > B200MOE_FP32) return B200ATTN_EINVAL;
+  if (tokens > 0 && logits == nullptr) return B200ATTN_EINVAL;
+  if (experts > kRouterMaxExperts || top_k > kRouterMaxTopK || top_k > experts || stride < 0) return B200ATTN_ESHAPE;
+  return reinterpret_cast<uintptr_t>(logits) % (dtype == B200MOE_FP32 ? 4 : 2) == 0 ? B200ATTN_OK : B200ATTN_EALIGN;
+}
+
+template <typename T, int VPL>
+void launch_router(const RouterArgs& a, cudaStream_t st) {
+  const int grid = (a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32);
+  if (a.bias != nullptr || a.groups > 1) router_topk_kernel<T, VPL, true><<<grid, kRouterThreads, 0, st>>>(a);
+  else router_topk_kernel<T, VPL, false><<<grid, kRouterThreads, 0, st>>>(a);
+}
+template <typename T, int VPL>
+void launch_router(const RouterBwdArgs& a, cudaStream_t st) {
+  router_topk_bwd_kernel<T, VPL><<<(a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32), kRouterThreads, 0, st>>>(a);
+}
+// by how many experts a lane holds
+template <typename T, typename Args>
+void launch_router_of(const Args& a, cudaStream_t st) {
+  if (a.experts <= 32) launch_router<T, 1>(a, st);
+  else if (a.experts <= 64) launch_router<T, 2>(a, st);
+  else if (a.experts <= 128) launch_router<T, 4>(a, st);
+  else launch_router<T, 8>(a, st);
+}
+template <typename Args>
+int launch_router_typed(const Args& a, int dtype, cudaStream_t st) {
+  if (dtype == B200MOE_BF16) launch_router_of<__nv_bfloat16>(a, st);
+  else if (dtype == B200MOE_FP16) launch_router_of<__half>(a, st);
+  else launch_router_of<float>(a, st);
+  return launch_status();
 }
 
 }  // namespace
@@ -228,6 +262,37 @@ int b200moe_route(const int64_t* indices, const float* weights, int32_t tokens, 
   moe_route_kernel<<<1, kRouteThreads, 0, st>>>(reinterpret_cast<const long long*>(indices), weights, (int)pairs, top_k, num_groups,
                                                    offsets, row_token, pos, row_weight);
   return launch_status();
+}
+
+int b200moe_router_topk(const void* logits, int64_t stride, const float* bias, void* weights, int64_t* indices, int32_t tokens,
+                        int32_t experts, int32_t top_k, int32_t groups, int32_t top_groups, int32_t sigmoid, int32_t renormalize,
+                        float scale, int32_t dtype, int32_t device, void* stream) {
+  int rc = check_router(logits, stride, tokens, experts, top_k, dtype);
+  if (rc) return rc;
+  if (groups <= 0 || top_groups <= 0 || (tokens > 0 && (weights == nullptr || indices == nullptr))) return B200ATTN_EINVAL;
+  if (groups > kRouterMaxGroups || experts % groups != 0 || top_groups > groups || top_k > experts / groups * top_groups) return B200ATTN_ESHAPE;
+  if ((rc = check_device(device))) return rc;
+  if (tokens == 0) return B200ATTN_OK;
+  DeviceGuard guard(device);
+  if (!guard.ok) return B200ATTN_ECUDA;
+  const RouterArgs a{logits, stride, bias, weights, reinterpret_cast<long long*>(indices), tokens, experts, top_k, groups, top_groups,
+                     sigmoid != 0, renormalize != 0, scale};
+  return launch_router_typed(a, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int b200moe_router_topk_bwd(const void* logits, int64_t stride, const int64_t* indices, const void* dweights, void* dlogits, int32_t tokens,
+                            int32_t experts, int32_t top_k, int32_t sigmoid, int32_t renormalize, float scale, int32_t dtype, int32_t device,
+                            void* stream) {
+  int rc = check_router(logits, stride, tokens, experts, top_k, dtype);
+  if (rc) return rc;
+  if (tokens > 0 && (indices == nullptr || dweights == nullptr || dlogits == nullptr)) return B200ATTN_EINVAL;
+  if ((rc = check_device(device))) return rc;
+  if (tokens == 0) return B200ATTN_OK;
+  DeviceGuard guard(device);
+  if (!guard.ok) return B200ATTN_ECUDA;
+  const RouterBwdArgs a{logits, stride, reinterpret_cast<const long long*>(indices), dweights, dlogits, tokens, experts, top_k,
+                        sigmoid != 0, renormalize != 0, scale};
+  return launch_router_typed(a, dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

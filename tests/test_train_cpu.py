@@ -140,3 +140,30 @@ def test_clip_refuses_bad_tensors():
         clip_grad_norm([q], 1.0)
     with pytest.raises(RuntimeError):
         global_grad_norm([p, q])
+
+
+def test_router_arguments_are_validated(lib):
+    buf = torch.zeros(1 << 10, dtype=torch.float32)
+    p = buf.data_ptr()
+
+    def fwd(l=p, stride=32, bias=None, w=p, i=p, T=2, E=32, k=4, groups=1, top=1, dtype=0):
+        return lib.b200moe_router_topk(l, stride, bias, w, i, T, E, k, groups, top, 0, 1, 1.0, dtype, 0, None)
+
+    def bwd(l=p, i=p, dw=p, dl=p, T=2, E=32, k=4, dtype=0):
+        return lib.b200moe_router_topk_bwd(l, 32, i, dw, dl, T, E, k, 0, 1, 1.0, dtype, 0, None)
+
+    assert fwd(l=None) == -1 and fwd(w=None) == -1 and fwd(i=None) == -1 and fwd(T=-1) == -1 and fwd(E=0) == -1 and fwd(k=0) == -1
+    assert fwd(dtype=3) == -1 and fwd(groups=0) == -1 and fwd(top=0) == -1
+    assert fwd(E=257) == -2 and fwd(k=33) == -2 and fwd(E=8, k=9) == -2 and fwd(stride=-1) == -2
+    assert fwd(groups=5) == -2 and fwd(groups=4, top=5) == -2 and fwd(E=256, groups=64) == -2 and fwd(groups=8, k=5, top=1) == -2
+    assert fwd(l=p + 1) == -4 and fwd(l=p + 2, dtype=2) == -4
+    assert bwd(l=None) == -1 and bwd(i=None) == -1 and bwd(dw=None) == -1 and bwd(dl=None) == -1 and bwd(dtype=-1) == -1
+    assert bwd(E=300) == -2 and bwd(E=3) == -2
+    if not torch.cuda.is_available():
+        assert fwd() in (-5, -6) and bwd() in (-5, -6)
+
+
+def test_router_refuses_cpu_tensors():
+    from oregon_gpt_oss_patching_b200.moe_router import router_topk
+    with pytest.raises(RuntimeError, match="needs CUDA tensors"):
+        router_topk(torch.zeros(3, 8), 2)
