@@ -27,44 +27,75 @@ int sm_count(int device) {
 int elem_size(int dtype) { return dtype == B200TRAIN_FP32 ? 4 : 2; }
 bool known_dtype(int dtype) { return dtype >= B200TRAIN_BF16 && dtype <= B200TRAIN_FP32; }
 
+// Launches a kernel that may start while the one before it in the stream runs out; it waits for that one's end itself.
+template <typename... P, typename... A>
+int launch_dependent(void (*kernel)(P...), unsigned grid, dim3 block, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid);
+  config.blockDim = block;
+  config.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess ? B200ATTN_OK : B200ATTN_ECUDA;
+}
+
 // ---------------------------------------------------------------- norm
 
-constexpr int kNormElems[] = {8, 16, 24, 32};   // elements a thread holds: the instances of the two kernels
+// Elements a thread holds: the instances of the two kernels, the preferred ones first (16-bit and 32-bit types).
+constexpr int kNormElems16[] = {24, 32, 16, 8}, kNormElems32[] = {16, 24, 32, 8};
+constexpr size_t kNormSmem = 216 * 1024;        // of a CTA's ring (static shared memory comes on top)
 
 struct NormShape {
   int elems = 0;     // one of kNormElems, 0: the row is too wide
   int threads = 0;   // of a row lane
   int lanes = 0;     // row lanes of a CTA
+  int grid = 0;
+  int stages = 0;    // of the ring
+  size_t smem = 0;
   bool shift = false;
 };
 
-// Where there are rows for every SM several times over, a thread takes as much of a row as it can hold (fewer threads
-// meet at a row's barrier); where there are not, a row is spread over as many threads as it has 8-element pieces.
-NormShape norm_shape(long long rows, int cols, int dtype, int device, int cta_threads) {
+// The piece of a row a thread that leaves the fewest threads without a word of it; where there are not rows enough for every
+// SM, the one that spreads a row over the most threads.  Then as many row lanes as there are threads and rows for, a ring of
+// three rows a lane where shared memory holds that for all of them, and of two otherwise.
+NormShape norm_shape(long long rows, int cols, int dtype, int device, int tensors) {
   NormShape s;
-  const int n = 16 / elem_size(dtype);
+  const int n = 16 / elem_size(dtype), sms = sm_count(device);
   s.shift = cols % n != 0;
   const int words = (cols + n - 1) / n + (s.shift ? 1 : 0);
-  const bool few = rows <= 2ll * sm_count(device);
-  for (int e : kNormElems) {
+  const bool few = rows <= sms;
+  long long held = 0;   // words that the threads of a row lane have room for
+  for (int e : dtype == B200TRAIN_FP32 ? kNormElems32 : kNormElems16) {
     const int per_thread = e / n;
-    const int threads = ((words + per_thread - 1) / per_thread + 31) / 32 * 32;
+    int threads = (words + per_thread - 1) / per_thread;
+    threads = threads <= 8 ? 8 : threads <= 16 ? 16 : (threads + 31) / 32 * 32;
     if (threads > kNormMaxThreads) continue;
+    if (s.elems != 0 && (few ? threads <= s.threads : (long long)threads * per_thread >= held)) continue;
     s.elems = e;
     s.threads = threads;
-    if (few || threads == 32) break;
+    held = (long long)threads * per_thread;
   }
   if (s.elems == 0) return s;
-  s.lanes = cta_threads / s.threads;
-  s.lanes = s.lanes < 1 ? 1 : (s.lanes > kNormMaxLanes ? kNormMaxLanes : s.lanes);
-  if (s.lanes > rows) s.lanes = rows < 1 ? 1 : (int)rows;
+  const size_t lane_stage = (size_t)s.threads * (s.elems / n) * 16 * tensors;   // bytes of one row of the ring
+  const size_t all = lane_stage * (kNormMaxThreads / s.threads);                 // of one row of every lane that has threads
+  s.stages = all * 3 <= kNormSmem ? 3 : lane_stage * 2 <= kNormSmem ? 2 : 1;
+  const int unit = s.threads < 32 ? 32 / s.threads : 1;   // lanes come in whole warps
+  int most = std::min((int)(kNormSmem / (lane_stage * s.stages)), kNormMaxThreads / s.threads);
+  if (s.threads > 32) most = std::min(most, kNormBarriers);
+  const long long spread = std::max(1ll, (rows + sms - 1) / sms);   // rows an SM
+  const int lanes = (int)std::min<long long>(most / unit * unit, (spread + unit - 1) / unit * unit);
+  s.lanes = lanes;
+  s.smem = lane_stage * s.stages * lanes;
+  const long long want = std::max(1ll, (rows + lanes - 1) / lanes);
+  s.grid = (int)std::min<long long>(want, sms);
+  if (s.shift && want > s.grid) {   // a lane's rows step by a multiple of 8 (see the kernels)
+    while (s.grid * lanes % 8 != 0 && s.grid > 1) --s.grid;
+    if (s.grid * lanes % 8 != 0) s.grid = 8;
+  }
   return s;
-}
-
-int norm_bwd_grid(const NormShape& s, long long rows, int device) {
-  const long long want = (rows + s.lanes - 1) / s.lanes, cap = sm_count(device);
-  const long long grid = want < cap ? want : cap;
-  return (int)((grid + 7) / 8 * 8);   // a lane's rows step by a multiple of 8 (see the kernel)
 }
 
 int check_norm_matrix(const void* p, int64_t stride, int64_t rows, int cols, int dtype) {
@@ -105,8 +136,6 @@ int with_shape(const NormShape& s, F f) {
     default: return s.shift ? f(Int<32 / N>{}, Int<1>{}) : f(Int<32 / N>{}, Int<0>{});
   }
 }
-
-constexpr int kFwdThreads = 256, kBwdThreads = 512;
 
 // ---------------------------------------------------------------- clip
 
@@ -227,21 +256,20 @@ int b200train_add_rms_norm(const void* x, int64_t x_stride, const void* residual
       ((rc = check_norm_matrix(residual, residual_stride, rows, cols, dtype)) || (rc = check_norm_matrix(h, cols, rows, cols, dtype))))
     return rc;
   if ((rc = check_device(device))) return rc;
-  const NormShape s = norm_shape(rows, cols, dtype, device, kFwdThreads);
+  const NormShape s = norm_shape(rows, cols, dtype, device, residual != nullptr ? 2 : 1);
   if (s.elems == 0) return B200ATTN_ESHAPE;
   if (rows == 0) return B200ATTN_OK;
-  const long long grid = (rows + s.lanes - 1) / s.lanes;
-  if (grid > 0x7fffffffll) return B200ATTN_ESHAPE;
   DeviceGuard guard(device);
   if (!guard.ok) return B200ATTN_ECUDA;
   return with_types(dtype, weight_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
     NormArgs<T, W> a{static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const W*>(weight), static_cast<T*>(y),
-                     static_cast<T*>(h), x_stride, residual_stride, rows, cols, eps};
+                     static_cast<T*>(h), x_stride, residual_stride, rows, cols, s.stages, eps};
     return with_shape<Elem<T>::N>(s, [&](auto vpt, auto shift) {
-      add_rms_norm_kernel<T, W, decltype(vpt)::value, decltype(shift)::value != 0>
-          <<<(unsigned)grid, dim3(s.threads, s.lanes), 0, static_cast<cudaStream_t>(stream)>>>(a);
+      constexpr auto kernel = add_rms_norm_kernel<T, W, decltype(vpt)::value, decltype(shift)::value != 0>;
+      if (int e = set_smem<kernel>(kNormSmem)) return e;
+      kernel<<<s.grid, dim3(s.threads, s.lanes), s.smem, static_cast<cudaStream_t>(stream)>>>(a);
       return launch_status();
     });
   });
@@ -249,8 +277,8 @@ int b200train_add_rms_norm(const void* x, int64_t x_stride, const void* residual
 
 int64_t b200train_norm_scratch_floats(int64_t rows, int32_t cols, int32_t dtype, int32_t device) {
   if (rows <= 0 || cols <= 0 || cols > B200TRAIN_NORM_MAX_COLS || !known_dtype(dtype)) return 0;
-  const NormShape s = norm_shape(rows, cols, dtype, device, kBwdThreads);
-  return s.elems == 0 ? 0 : (int64_t)norm_bwd_grid(s, rows, device) * cols;
+  // (a pass without dh may take more row lanes a CTA, never more CTAs than there are SMs)
+  return (int64_t)std::min<int64_t>(rows, std::max(sm_count(device), 8)) * cols;
 }
 
 int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
@@ -264,7 +292,7 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
     return rc;
   if (dh != nullptr && (rc = check_norm_matrix(dh, dh_stride, rows, cols, dtype))) return rc;
   if ((rc = check_device(device))) return rc;
-  const NormShape s = norm_shape(rows, cols, dtype, device, kBwdThreads);
+  const NormShape s = norm_shape(rows, cols, dtype, device, dh != nullptr ? 3 : 2);
   if (s.elems == 0) return B200ATTN_ESHAPE;
   DeviceGuard guard(device);
   if (!guard.ok) return B200ATTN_ECUDA;
@@ -272,23 +300,21 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
   if (rows == 0)
     return dweight == nullptr || cudaMemsetAsync(dweight, 0, (size_t)cols * elem_size(weight_dtype), st) == cudaSuccess ? B200ATTN_OK
                                                                                                                          : B200ATTN_ECUDA;
-  const int grid = norm_bwd_grid(s, rows, device);
-  if (dweight != nullptr && (scratch == nullptr || scratch_floats < (int64_t)grid * cols)) return B200ATTN_ESCRATCH;
+  if (dweight != nullptr && (scratch == nullptr || scratch_floats < (int64_t)s.grid * cols)) return B200ATTN_ESCRATCH;
   return with_types(dtype, weight_dtype, [&](auto t, auto w) {
     using T = decltype(t);
     using W = decltype(w);
     NormBwdArgs<T, W> a{static_cast<const T*>(dy), static_cast<const T*>(dh), static_cast<const T*>(h), static_cast<const W*>(weight),
-                        static_cast<T*>(dx), dweight != nullptr ? scratch : nullptr, dy_stride, dh_stride, h_stride, rows, cols, eps};
+                        static_cast<T*>(dx), dweight != nullptr ? scratch : nullptr, dy_stride, dh_stride, h_stride, rows, cols, s.stages, eps};
     int rc2 = with_shape<Elem<T>::N>(s, [&](auto vpt, auto shift) {
       constexpr auto kernel = add_rms_norm_bwd_kernel<T, W, decltype(vpt)::value, decltype(shift)::value != 0>;
-      const size_t smem = (size_t)s.lanes * cols * sizeof(float);
-      if (int e = set_smem<kernel>(kNormMaxThreads * 32 * sizeof(float))) return e;
-      kernel<<<grid, dim3(s.threads, s.lanes), smem, st>>>(a);
+      if (int e = set_smem<kernel>(kNormSmem)) return e;
+      kernel<<<s.grid, dim3(s.threads, s.lanes), s.smem, st>>>(a);
       return launch_status();
     });
     if (rc2 || dweight == nullptr) return rc2;
-    norm_dw_kernel<W><<<(cols + 31) / 32, dim3(32, 32), 0, st>>>(scratch, static_cast<W*>(dweight), grid, cols);
-    return launch_status();
+    return launch_dependent(norm_dw_kernel<W>, (cols + 31) / 32, dim3(32, 32), st, static_cast<const float*>(scratch), static_cast<W*>(dweight),
+                            s.grid, cols);
   });
 }
 

@@ -7,6 +7,34 @@
 
 namespace b200train {
 
+// Two fp32 values in one 64-bit register pair: sm_100 adds, multiplies and multiply-adds both in one instruction.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 make2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 split2(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // Elem<T>: N elements fill 16 bytes; unpack / pack convert a whole 16-byte word, load1 / store1 a single element.
 template <typename T>
 struct Elem;
@@ -75,6 +103,26 @@ __device__ __forceinline__ uint4 pack(const float* f) {
   } else {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   }
+}
+
+// The same with the elements in pairs: N / 2 of them fill 16 bytes.
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, F2* f) {
+  float e[Elem<T>::N];
+  unpack<T>(v, e);
+#pragma unroll
+  for (int i = 0; i < Elem<T>::N / 2; ++i) f[i] = make2(e[2 * i], e[2 * i + 1]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const F2* f) {
+  float e[Elem<T>::N];
+#pragma unroll
+  for (int i = 0; i < Elem<T>::N / 2; ++i) {
+    const float2 p = split2(f[i]);
+    e[2 * i] = p.x;
+    e[2 * i + 1] = p.y;
+  }
+  return pack<T>(e);
 }
 
 }  // namespace b200train

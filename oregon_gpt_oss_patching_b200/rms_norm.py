@@ -18,10 +18,10 @@ every sum is fixed by the sizes, so results are bit-reproducible.  Rows of up to
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _cabi
 
@@ -49,79 +49,87 @@ def _check(name, x, residual, weight, eps):
 
 
 def _rows(t, cols):
-    """``t`` as (rows, cols) with a row stride the kernels can address in place, else a contiguous copy."""
-    if t.is_contiguous():
-        t = t.view(-1, cols)
-    else:
+    """``(tensor, row stride)`` that the kernels can address in place: ``t`` itself, rows of a view of it, or a contiguous copy."""
+    if not t.is_contiguous():
         t = t.reshape(-1, cols)
         per_word = 16 // t.element_size()
-        if t.stride(1) != 1 or cols % per_word or t.stride(0) % per_word:
+        if t.is_contiguous() or t.stride(1) != 1 or cols % per_word or t.stride(0) % per_word:
             t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]   # (a single row may carry any stride)
+        elif t.data_ptr() % 16 == 0:
+            return t, t.stride(0)
+    return (t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)), cols
 
 
 def _forward(x, residual, weight, eps):
-    """x, residual: (rows, cols); returns (y, h), h None without a residual."""
-    rows, cols = x.shape
-    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    h = None if residual is None else torch.empty_like(y)
-    rc = _cabi.load().b200train_add_rms_norm(
-        x.data_ptr(), _stride(x), None if residual is None else residual.data_ptr(), 0 if residual is None else _stride(residual),
-        weight.data_ptr(), y.data_ptr(), None if h is None else h.data_ptr(), rows, cols, eps, _cabi.TRAIN_DTYPES[x.dtype],
-        _cabi.TRAIN_DTYPES[weight.dtype], x.device.index, torch.cuda.current_stream(x.device).cuda_stream)
+    """Returns (y, h, weight, what the backward reads as h, its row stride); h is None without a residual."""
+    cols = x.shape[-1]
+    xr, x_stride = _rows(x, cols)
+    w = weight if weight.is_contiguous() and weight.data_ptr() % 16 == 0 else weight.clone(memory_format=torch.contiguous_format)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dev = x.get_device()
+    if residual is None:
+        h, kept, kept_stride, r_ptr, r_stride, h_ptr = None, xr, x_stride, None, 0, None
+    else:
+        r, r_stride = _rows(residual, cols)
+        h = torch.empty_like(y)
+        kept, kept_stride, r_ptr, h_ptr = h, cols, r.data_ptr(), h.data_ptr()
+    rc = _cabi.load().b200train_add_rms_norm(xr.data_ptr(), x_stride, r_ptr, r_stride, w.data_ptr(), y.data_ptr(), h_ptr, x.numel() // cols, cols,
+                                             eps, _cabi.TRAIN_DTYPES[x.dtype], _cabi.TRAIN_DTYPES[w.dtype], dev, _cabi.stream_of(dev))
     _cabi.check(rc, "b200train_add_rms_norm")
-    return y, h
+    return y, h, w, kept, kept_stride
 
 
-def _weight(weight):
-    weight = weight.contiguous()
-    return weight if weight.data_ptr() % 16 == 0 else weight.clone()
+@lru_cache(maxsize=1024)
+def _scratch_floats(rows, cols, dtype, dev):
+    return _cabi.load().b200train_norm_scratch_floats(rows, cols, dtype, dev)
 
 
 class _add_rms_norm(torch.autograd.Function):
-    """forward(x, residual or None, weight, eps) -> (y, h): h is the sum, or x itself where there is no residual."""
+    """forward(x, residual or None, weight, eps, passed) -> (y, h): h is the sum; without a residual x itself if `passed`, or None."""
 
     @staticmethod
-    def forward(ctx, x, residual, weight, eps):
-        cols = x.shape[-1]
-        x2, w = _rows(x, cols), _weight(weight)
-        y, h = _forward(x2, None if residual is None else _rows(residual, cols), w, eps)
-        ctx.save_for_backward(x2 if h is None else h, w)
+    def forward(ctx, x, residual, weight, eps, passed):
+        y, h, w, kept, ctx.h_stride = _forward(x, residual, weight, eps)
+        if kept is h:       # (an output saved as it is would keep itself alive; a view shares its memory and its version)
+            kept = h.detach()
+        elif kept is x:
+            kept = x.detach()
+        ctx.save_for_backward(kept, w)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
-        return y.view(x.shape), x if h is None else h.view(x.shape)
+        return y, (x if passed else None) if h is None else h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh):
-        h, w = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            raise RuntimeError("add_rms_norm cannot be differentiated twice")
         if dy is None:      # the norm was not used: the stream's gradient passes through
-            return dh, dh if ctx.needs_input_grad[1] else None, None, None
-        rows, cols = h.shape
-        shape = dy.shape
-        dy = _rows(dy, cols)
-        if dh is not None:
-            dh = _rows(dh, cols)
-        lib = _cabi.load()
-        dt, dev = _cabi.TRAIN_DTYPES[h.dtype], h.device
-        dx = torch.empty((rows, cols), dtype=h.dtype, device=dev)
+            return dh, dh if ctx.needs_input_grad[1] else None, None, None, None
+        h, w = ctx.saved_tensors
+        cols = w.shape[0]
+        rows = dy.numel() // cols
+        wants = ctx.needs_input_grad
+        dyr, dy_stride = _rows(dy, cols)
+        dhr, dh_stride = (None, 0) if dh is None else _rows(dh, cols)
+        dev = dy.get_device()
+        dt = _cabi.TRAIN_DTYPES[dy.dtype]
+        dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
         dw = scratch = None
         floats = 0
-        if ctx.needs_input_grad[2]:
+        if wants[2]:
             dw = torch.empty_like(w)
-            floats = lib.b200train_norm_scratch_floats(rows, cols, dt, dev.index)
-            scratch = torch.empty(floats, dtype=torch.float32, device=dev)
-        rc = lib.b200train_add_rms_norm_bwd(
-            dy.data_ptr(), _stride(dy), None if dh is None else dh.data_ptr(), 0 if dh is None else _stride(dh), h.data_ptr(), _stride(h),
-            w.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(), None if scratch is None else scratch.data_ptr(), floats, rows,
-            cols, ctx.eps, dt, _cabi.TRAIN_DTYPES[w.dtype], dev.index, torch.cuda.current_stream(dev).cuda_stream)
+            floats = _scratch_floats(rows, cols, dt, dev)
+            scratch = torch.empty(floats, dtype=torch.float32, device=dy.device)
+        rc = _cabi.load().b200train_add_rms_norm_bwd(
+            dyr.data_ptr(), dy_stride, None if dhr is None else dhr.data_ptr(), dh_stride, h.data_ptr(), ctx.h_stride, w.data_ptr(),
+            dx.data_ptr(), None if dw is None else dw.data_ptr(), None if scratch is None else scratch.data_ptr(), floats, rows, cols, ctx.eps,
+            dt, _cabi.TRAIN_DTYPES[w.dtype], dev, _cabi.stream_of(dev))
         _cabi.check(rc, "b200train_add_rms_norm_bwd")
-        dx = dx.view(shape)
-        return dx, dx if ctx.needs_input_grad[1] else None, dw, None
+        return dx, dx if wants[1] else None, dw, None, None
+
+
+def _differentiates(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5):
@@ -130,14 +138,21 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     With ``residual=None`` h is ``x`` itself: passing the stream through the norm this way lets the backward add the
     stream's gradient in the same kernel.
     """
+    eps = float(eps)
     _check("add_rms_norm", x, residual, weight, eps)
-    return _add_rms_norm.apply(x, residual, weight, float(eps))
+    if _differentiates(x, residual, weight):
+        return _add_rms_norm.apply(x, residual, weight, eps, True)
+    y, h, _, _, _ = _forward(x, residual, weight, eps)
+    return y, x if h is None else h
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
     """The RMS norm of ``x`` over its last dimension, times ``weight``."""
+    eps = float(eps)
     _check("rms_norm", x, None, weight, eps)
-    return _add_rms_norm.apply(x, None, weight, float(eps))[0]
+    if _differentiates(x, weight):
+        return _add_rms_norm.apply(x, None, weight, eps, False)[0]
+    return _forward(x, None, weight, eps)[0]
 
 
 def b200_rms_norm_forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
