@@ -65,14 +65,25 @@ int check_router(const void* logits, int64_t stride, int tokens, int experts, in
   return reinterpret_cast<uintptr_t>(logits) % (dtype == B200MOE_FP32 ? 4 : 2) == 0 ? B200ATTN_OK : B200ATTN_EALIGN;
 }
 
+// Whether runs of `run` elements that start at p, p + stride, ... lie on a grid of their size (16 bytes where they are longer).
+bool on_grid(const void* p, int64_t stride, int run, int size) {
+  const int64_t bytes = run * size > 16 ? 16 : run * size;
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0;
+}
+
 template <typename T, int VPL>
-void launch_router(const RouterArgs& a, cudaStream_t st) {
+void launch_router(RouterArgs a, cudaStream_t st) {
+  const bool exact = sizeof(T) == 2 && a.bias == nullptr && a.groups == 1;
+  a.slow = !exact && (a.top_k >= 32 || (a.groups & (a.groups - 1)) != 0);
+  a.vector = a.experts == 32 * VPL && on_grid(a.logits, a.stride, VPL, sizeof(T));   // (every lane holds VPL neighbours)
   const int grid = (a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32);
   if (a.bias != nullptr || a.groups > 1) router_topk_kernel<T, VPL, true><<<grid, kRouterThreads, 0, st>>>(a);
   else router_topk_kernel<T, VPL, false><<<grid, kRouterThreads, 0, st>>>(a);
 }
 template <typename T, int VPL>
-void launch_router(const RouterBwdArgs& a, cudaStream_t st) {
+void launch_router(RouterBwdArgs a, cudaStream_t st) {
+  a.vector_in = on_grid(a.logits, a.stride, VPL, sizeof(T));
+  a.vector_out = on_grid(a.dlogits, a.experts, VPL, sizeof(T));
   router_topk_bwd_kernel<T, VPL><<<(a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32), kRouterThreads, 0, st>>>(a);
 }
 // by how many experts a lane holds
@@ -276,7 +287,7 @@ int b200moe_router_topk(const void* logits, int64_t stride, const float* bias, v
   DeviceGuard guard(device);
   if (!guard.ok) return B200ATTN_ECUDA;
   const RouterArgs a{logits, stride, bias, weights, reinterpret_cast<long long*>(indices), tokens, experts, top_k, groups, top_groups,
-                     sigmoid != 0, renormalize != 0, scale};
+                     sigmoid != 0, renormalize != 0, 0, 0, scale};
   return launch_router_typed(a, dtype, static_cast<cudaStream_t>(stream));
 }
 
@@ -291,7 +302,7 @@ int b200moe_router_topk_bwd(const void* logits, int64_t stride, const int64_t* i
   DeviceGuard guard(device);
   if (!guard.ok) return B200ATTN_ECUDA;
   const RouterBwdArgs a{logits, stride, reinterpret_cast<const long long*>(indices), dweights, dlogits, tokens, experts, top_k,
-                        sigmoid != 0, renormalize != 0, scale};
+                        sigmoid != 0, renormalize != 0, 0, 0, scale};
   return launch_router_typed(a, dtype, static_cast<cudaStream_t>(stream));
 }
 
