@@ -166,11 +166,6 @@ def check(code: int, what: str) -> None:
         raise RuntimeError(f"{what} failed: {strerror(code)} (code {code})")
 
 
-def stream_of(device_index: int) -> int:
-    """The current stream's handle: ``torch.cuda.current_stream(device).cuda_stream`` without the object, a thirtieth of its time."""
-    return torch._C._cuda_getCurrentRawStream(device_index)
-
-
 def padded_len(S: int) -> int:
     return (int(S) + ROW_TILE - 1) // ROW_TILE * ROW_TILE
 

@@ -1,0 +1,418 @@
+// The training-step operators as torch functions: argument checks, allocations and autograd around the C ABI of
+// include/b200train.h and the router of include/b200moe.h.  Host code alone, one extension module.
+//
+// The attention and expert wrappers do this in Python; these operators are called once or twice a layer on little data (or on
+// hundreds of small tensors), where the host's time is what a caller waits for: a norm of a few rows takes 9 us of it here and 14 us
+// through Python and ctypes, a forward with its backward 62 us and 94 us (45 us of them autograd's own), the routing of a few
+// tokens 7 us and 22 us, clipping 48 gradients 20 us and 50 us.
+//
+// The module calls the library through addresses it is given (set_library), so that there is one loaded copy of it, the one
+// that the Python side found, checked and reports on.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <limits>
+#include <optional>
+#include <string>
+#include <unordered_map>
+#include <vector>
+
+#include "../../include/b200moe.h"
+#include "../../include/b200train.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Library {
+  decltype(&b200attn_strerror) strerror = nullptr;
+  decltype(&b200train_add_rms_norm) add_rms_norm = nullptr;
+  decltype(&b200train_norm_scratch_floats) norm_scratch_floats = nullptr;
+  decltype(&b200train_add_rms_norm_bwd) add_rms_norm_bwd = nullptr;
+  decltype(&b200train_clip_scratch_doubles) clip_scratch_doubles = nullptr;
+  decltype(&b200train_grad_norm) grad_norm = nullptr;
+  decltype(&b200train_clip_grads) clip_grads = nullptr;
+  decltype(&b200train_clipped_sgd) clipped_sgd = nullptr;
+  decltype(&b200moe_router_topk) router_topk = nullptr;
+  decltype(&b200moe_router_topk_bwd) router_topk_bwd = nullptr;
+} lib;
+
+template <typename F>
+void take_address(F& f, const std::unordered_map<std::string, uintptr_t>& addresses, const char* name) {
+  const auto at = addresses.find(name);
+  TORCH_CHECK(at != addresses.end() && at->second != 0, "libb200attn.so has no ", name);
+  f = reinterpret_cast<F>(at->second);
+}
+
+void set_library(const std::unordered_map<std::string, uintptr_t>& a) {
+  take_address(lib.strerror, a, "b200attn_strerror");
+  take_address(lib.add_rms_norm, a, "b200train_add_rms_norm");
+  take_address(lib.norm_scratch_floats, a, "b200train_norm_scratch_floats");
+  take_address(lib.add_rms_norm_bwd, a, "b200train_add_rms_norm_bwd");
+  take_address(lib.clip_scratch_doubles, a, "b200train_clip_scratch_doubles");
+  take_address(lib.grad_norm, a, "b200train_grad_norm");
+  take_address(lib.clip_grads, a, "b200train_clip_grads");
+  take_address(lib.clipped_sgd, a, "b200train_clipped_sgd");
+  take_address(lib.router_topk, a, "b200moe_router_topk");
+  take_address(lib.router_topk_bwd, a, "b200moe_router_topk_bwd");
+}
+
+void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed: ", lib.strerror(rc), " (code ", rc, ")"); }
+
+// B200TRAIN_* and B200MOE_* (the same numbers), -1 for any other type
+int dtype_code(at::ScalarType t) {
+  switch (t) {
+    case at::kBFloat16: return B200TRAIN_BF16;
+    case at::kHalf: return B200TRAIN_FP16;
+    case at::kFloat: return B200TRAIN_FP32;
+    default: return -1;
+  }
+}
+
+void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+Tensor copy_of(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+// ---------------------------------------------------------------- norm
+
+// Rows that the kernels can address in place (`t` itself or a view of it), or a contiguous copy, with the row stride.
+struct Rows {
+  Tensor t;
+  int64_t stride;
+  Rows() : stride(0) {}
+  Rows(const Tensor& of, int64_t cols) : t(of), stride(cols) {
+    if (!t.is_contiguous()) {
+      t = t.reshape({-1, cols});
+      const int64_t per_word = 16 / static_cast<int64_t>(t.element_size());
+      if (!t.is_contiguous()) {
+        if (t.stride(1) != 1 || cols % per_word != 0 || t.stride(0) % per_word != 0) t = t.contiguous();
+        else stride = t.stride(0);
+      }
+    }
+    if (!aligned16(t)) {
+      t = copy_of(t);
+      stride = cols;
+    }
+  }
+};
+
+void check_norm(const char* name, const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, double eps) {
+  TORCH_CHECK(x.is_cuda(), name, " needs CUDA tensors (the sm_100a library is the only code path)");
+  TORCH_CHECK_TYPE(dtype_code(x.scalar_type()) >= 0, name, " supports bfloat16, float16 and float32, got ", x.dtype());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, name, ": x must have a last dimension to normalise, got shape ", x.sizes());
+  TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == x.size(-1), name, ": weight must be (", x.size(-1), ",), got ", weight.sizes());
+  TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat, name, ": weight must be ", x.dtype(),
+                   " or float32, got ", weight.dtype());
+  TORCH_CHECK(weight.device() == x.device(), name, ": weight is on ", weight.device(), ", x on ", x.device());
+  if (residual.has_value())
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type() && residual->device() == x.device(), name,
+                      ": residual must match x (", x.sizes(), ", ", x.dtype(), ", ", x.device(), "), got ", residual->sizes(), ", ",
+                      residual->dtype(), ", ", residual->device());
+  TORCH_CHECK_VALUE(eps >= 0.0, name, ": eps must not be negative, got ", eps);
+  TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int32_t>::max(), name, ": rows of ", x.size(-1), " elements");
+}
+
+struct Normed {
+  Tensor y, h;      // h undefined without a residual
+  Rows kept;        // what the backward reads as h
+  Tensor weight;
+};
+
+Normed norm_forward(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, double eps) {
+  const int64_t cols = x.size(-1);
+  const int device = x.get_device();
+  Normed n;
+  const Rows in(x, cols);
+  n.weight = weight.is_contiguous() && aligned16(weight) ? weight : copy_of(weight);
+  n.y = at::empty(x.sizes(), x.options());
+  Rows r;
+  if (residual.has_value()) {
+    r = Rows(*residual, cols);
+    n.h = at::empty(x.sizes(), x.options());
+    n.kept.t = n.h;
+    n.kept.stride = cols;
+  } else {
+    n.kept = in;
+  }
+  check(lib.add_rms_norm(data(in.t), in.stride, data(r.t), r.stride, data(n.weight), n.y.mutable_data_ptr(),
+                         n.h.defined() ? n.h.mutable_data_ptr() : nullptr, x.numel() / cols, static_cast<int32_t>(cols),
+                         static_cast<float>(eps), dtype_code(x.scalar_type()), dtype_code(n.weight.scalar_type()), device, stream_of(device)),
+        "b200train_add_rms_norm");
+  return n;
+}
+
+// forward(x, residual or none, weight, eps, passed) -> (y, h): h is the sum; without a residual x itself if `passed`, or y alone.
+struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, double eps,
+                               bool passed) {
+    Normed n = norm_forward(x, residual, weight, eps);
+    ctx->save_for_backward({n.kept.t, n.weight});
+    ctx->saved_data["stride"] = n.kept.stride;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["residual"] = residual.has_value();
+    ctx->set_materialize_grads(false);
+    if (n.h.defined()) return {n.y, n.h};
+    if (passed) return {n.y, x};
+    return {n.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "add_rms_norm cannot be differentiated twice");
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
+    const Tensor none;
+    if (!dy.defined()) return {dh, residual ? dh : none, none, none, none};   // the norm was not used: the stream's gradient passes through
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &w = saved[1];
+    const int64_t cols = w.size(0), rows = dy.numel() / cols;
+    const int device = dy.get_device(), dtype = dtype_code(dy.scalar_type());
+    const Rows dyr(dy, cols), dhr = dh.defined() ? Rows(dh, cols) : Rows();
+    Tensor dx = at::empty(dy.sizes(), dy.options()), dw, scratch;
+    int64_t floats = 0;
+    if (ctx->needs_input_grad(residual ? 2 : 1)) {   // (an input that is not there has no place)
+      dw = at::empty(w.sizes(), w.options());
+      floats = lib.norm_scratch_floats(rows, static_cast<int32_t>(cols), dtype, device);
+      scratch = at::empty({floats}, dy.options().dtype(at::kFloat));
+    }
+    check(lib.add_rms_norm_bwd(data(dyr.t), dyr.stride, data(dhr.t), dhr.stride, data(h), ctx->saved_data["stride"].toInt(), data(w),
+                               dx.mutable_data_ptr(), dw.defined() ? dw.mutable_data_ptr() : nullptr,
+                               scratch.defined() ? scratch.mutable_data_ptr<float>() : nullptr, floats, rows, static_cast<int32_t>(cols),
+                               static_cast<float>(ctx->saved_data["eps"].toDouble()), dtype, dtype_code(w.scalar_type()), device,
+                               stream_of(device)),
+          "b200train_add_rms_norm_bwd");
+    return {dx, residual ? dx : none, dw, none, none};
+  }
+};
+
+bool differentiates(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight) {
+  return at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (residual.has_value() && residual->requires_grad()));
+}
+
+std::pair<Tensor, Tensor> add_rms_norm(const Tensor& x, const std::optional<Tensor>& residual, const Tensor& weight, double eps) {
+  check_norm("add_rms_norm", x, residual, weight, eps);
+  if (differentiates(x, residual, weight)) {
+    variable_list out = AddRmsNorm::apply(x, residual, weight, eps, true);
+    return {out[0], out[1]};
+  }
+  Normed n = norm_forward(x, residual, weight, eps);
+  return {n.y, n.h.defined() ? n.h : x};
+}
+
+Tensor rms_norm(const Tensor& x, const Tensor& weight, double eps) {
+  check_norm("rms_norm", x, std::nullopt, weight, eps);
+  if (differentiates(x, std::nullopt, weight)) return AddRmsNorm::apply(x, std::nullopt, weight, eps, false)[0];
+  return norm_forward(x, std::nullopt, weight, eps).y;
+}
+
+// ---------------------------------------------------------------- router
+
+struct Routing {
+  int64_t top_k, num_groups, top_groups;
+  bool sigmoid, renormalize;
+  double scale;
+};
+
+std::pair<Tensor, Tensor> router_forward(const Tensor& logits, const std::optional<Tensor>& bias, const Routing& how) {
+  const int device = logits.get_device();
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  Tensor b;
+  if (bias.has_value()) b = bias->detach().to(at::kFloat).contiguous();
+  Tensor weights = at::empty({tokens, how.top_k}, logits.options());
+  Tensor indices = at::empty({tokens, how.top_k}, logits.options().dtype(at::kLong));
+  check(lib.router_topk(data(logits), logits.stride(0), b.defined() ? b.const_data_ptr<float>() : nullptr, weights.mutable_data_ptr(),
+                        indices.mutable_data_ptr<int64_t>(), static_cast<int32_t>(tokens), static_cast<int32_t>(experts),
+                        static_cast<int32_t>(how.top_k), static_cast<int32_t>(how.num_groups), static_cast<int32_t>(how.top_groups), how.sigmoid,
+                        how.renormalize, static_cast<float>(how.scale), dtype_code(logits.scalar_type()), device, stream_of(device)),
+        "b200moe_router_topk");
+  return {weights, indices};
+}
+
+// A row's elements lie next to each other.
+Tensor row_major(const Tensor& logits) { return logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous(); }
+
+struct RouterTopk : torch::autograd::Function<RouterTopk> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& given, const std::optional<Tensor>& bias, int64_t top_k, int64_t num_groups,
+                               int64_t top_groups, bool sigmoid, bool renormalize, double scale) {
+    const Tensor logits = row_major(given);
+    auto [weights, indices] = router_forward(logits, bias, {top_k, num_groups, top_groups, sigmoid, renormalize, scale});
+    ctx->save_for_backward({logits, indices});
+    ctx->mark_non_differentiable({indices});
+    ctx->saved_data["sigmoid"] = sigmoid;
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return {weights, indices};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "router_topk cannot be differentiated twice");
+    variable_list out(8);
+    if (!grads[0].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &indices = saved[1], dweights = grads[0].contiguous();
+    const int device = logits.get_device();
+    out[0] = at::empty(logits.sizes(), logits.options());
+    check(lib.router_topk_bwd(data(logits), logits.stride(0), indices.const_data_ptr<int64_t>(), data(dweights), out[0].mutable_data_ptr(),
+                              static_cast<int32_t>(logits.size(0)), static_cast<int32_t>(logits.size(1)), static_cast<int32_t>(indices.size(1)),
+                              ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renormalize"].toBool(),
+                              static_cast<float>(ctx->saved_data["scale"].toDouble()), dtype_code(logits.scalar_type()), device,
+                              stream_of(device)),
+          "b200moe_router_topk_bwd");
+    return out;
+  }
+};
+
+std::pair<Tensor, Tensor> router_topk(const Tensor& logits, int64_t top_k, const std::string& scoring, const std::optional<Tensor>& bias,
+                                      int64_t num_groups, int64_t top_groups, bool renormalize, double scale) {
+  TORCH_CHECK(logits.is_cuda(), "router_topk needs CUDA tensors (the sm_100a library is the only code path)");
+  TORCH_CHECK_TYPE(dtype_code(logits.scalar_type()) >= 0, "router_topk supports bfloat16, float16 and float32 logits, got ", logits.dtype());
+  TORCH_CHECK_VALUE(logits.dim() == 2, "router_topk: logits must be (tokens, experts), got ", logits.sizes());
+  TORCH_CHECK_VALUE(scoring == "softmax" || scoring == "sigmoid", "router_topk: scoring must be 'softmax' or 'sigmoid', got '", scoring, "'");
+  const int64_t experts = logits.size(1);
+  TORCH_CHECK_VALUE(experts >= 1 && experts <= B200MOE_ROUTER_MAX_EXPERTS, "router_topk: 1 to ", B200MOE_ROUTER_MAX_EXPERTS, " experts, got ", experts);
+  TORCH_CHECK_VALUE(num_groups >= 1 && num_groups <= B200MOE_ROUTER_MAX_GROUPS && experts % num_groups == 0 && top_groups >= 1 &&
+                        top_groups <= num_groups,
+                    "router_topk: ", experts, " experts cannot form ", num_groups, " equal groups of which ", top_groups, " are eligible");
+  const int64_t eligible = experts / num_groups * top_groups;
+  TORCH_CHECK_VALUE(top_k >= 1 && top_k <= std::min<int64_t>(B200MOE_ROUTER_MAX_TOP_K, eligible), "router_topk: cannot choose ", top_k, " of ",
+                    eligible, " eligible experts (at most ", B200MOE_ROUTER_MAX_TOP_K, ")");
+  TORCH_CHECK_VALUE(logits.size(0) <= std::numeric_limits<int32_t>::max(), "router_topk: ", logits.size(0), " tokens");
+  if (bias.has_value())
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == experts && bias->device() == logits.device() && bias->is_floating_point(),
+                      "router_topk: bias must be ", experts, " floating point values on ", logits.device());
+  const bool sigmoid = scoring == "sigmoid";
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    const std::optional<Tensor> b = bias.has_value() ? std::optional<Tensor>(bias->detach()) : std::nullopt;   // the choice has no gradient
+    variable_list out = RouterTopk::apply(logits, b, top_k, num_groups, top_groups, sigmoid, renormalize, scale);
+    return {out[0], out[1]};
+  }
+  return router_forward(row_major(logits), bias, {top_k, num_groups, top_groups, sigmoid, renormalize, scale});
+}
+
+// ---------------------------------------------------------------- clip
+
+// The arrays that the library reads: addresses, counts and types of contiguous tensors on one device.
+struct Table {
+  std::vector<int64_t> grads, params, counts;
+  std::vector<int32_t> dtypes;
+  int device = -1;
+  Table(const char* name, const std::vector<Tensor>& g, const std::vector<Tensor>* p) {
+    const size_t n = g.size();
+    grads.resize(n);
+    counts.resize(n);
+    dtypes.resize(n);
+    if (p != nullptr) params.resize(n);
+    device = g[0].is_cuda() ? static_cast<int>(g[0].get_device()) : -1;
+    for (size_t i = 0; i < n; ++i) {
+      TORCH_CHECK(device >= 0 && g[i].is_cuda() && g[i].get_device() == device && (p == nullptr || ((*p)[i].is_cuda() && (*p)[i].get_device() == device)),
+                  name, " needs CUDA tensors on one device (the sm_100a library is the only code path)");
+      TORCH_CHECK_TYPE(g[i].layout() == at::kStrided, name, " supports strided tensors, got ", g[i].layout());
+      dtypes[i] = dtype_code(g[i].scalar_type());
+      TORCH_CHECK_TYPE(dtypes[i] >= 0, name, " supports bfloat16, float16 and float32, got ", g[i].dtype());
+      counts[i] = g[i].numel();
+      grads[i] = reinterpret_cast<int64_t>(g[i].const_data_ptr());
+      if (p != nullptr) params[i] = reinterpret_cast<int64_t>((*p)[i].const_data_ptr());
+    }
+  }
+};
+
+struct Output {
+  Tensor scratch, norm;
+  int64_t doubles;
+  Output(const Tensor& like, size_t tensors, int device) {
+    doubles = lib.clip_scratch_doubles(static_cast<int64_t>(tensors), device);
+    scratch = at::empty({doubles}, like.options().dtype(at::kDouble));
+    norm = at::empty({}, like.options().dtype(at::kFloat));
+  }
+};
+
+Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+
+float limit_of(const char* name, double max_norm) {
+  TORCH_CHECK_VALUE(max_norm >= 0.0, name, ": max_norm must not be negative, got ", max_norm);
+  return static_cast<float>(max_norm);
+}
+
+Tensor global_grad_norm(const std::vector<Tensor>& tensors) {
+  at::NoGradGuard no_grad;
+  if (tensors.empty()) return at::zeros({}, at::kFloat);
+  std::vector<Tensor> packed;
+  packed.reserve(tensors.size());
+  for (const Tensor& t : tensors) packed.push_back(dense(t));
+  const Table t("global_grad_norm", packed, nullptr);
+  Output out(packed[0], packed.size(), t.device);
+  check(lib.grad_norm(t.grads.data(), t.counts.data(), t.dtypes.data(), static_cast<int64_t>(packed.size()), out.scratch.mutable_data_ptr<double>(),
+                      out.doubles, out.norm.mutable_data_ptr<float>(), t.device, stream_of(t.device)),
+        "b200train_grad_norm");
+  return out.norm;
+}
+
+Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm) {
+  at::NoGradGuard no_grad;
+  const float limit = limit_of("clip_grad_norm", max_norm);
+  std::vector<Tensor> grads, packed;
+  grads.reserve(parameters.size());
+  packed.reserve(parameters.size());
+  for (const Tensor& p : parameters) {
+    const Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    for (int64_t d = 0; d < g.dim(); ++d)
+      TORCH_CHECK_VALUE(g.layout() != at::kStrided || g.stride(d) != 0 || g.size(d) <= 1,
+                        "clip_grad_norm: a gradient with a stride of 0 cannot be scaled in place");
+    grads.push_back(g);
+    packed.push_back(g.layout() == at::kStrided ? dense(g) : g);
+  }
+  if (grads.empty()) return at::zeros({}, at::kFloat);
+  const Table t("clip_grad_norm", packed, nullptr);
+  Output out(packed[0], packed.size(), t.device);
+  check(lib.clip_grads(t.grads.data(), t.counts.data(), t.dtypes.data(), static_cast<int64_t>(packed.size()), limit,
+                       out.scratch.mutable_data_ptr<double>(), out.doubles, out.norm.mutable_data_ptr<float>(), t.device, stream_of(t.device)),
+        "b200train_clip_grads");
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (packed[i].is_same(grads[i])) grads[i].unsafeGetTensorImpl()->bump_version();
+    else grads[i].copy_(packed[i]);
+  }
+  return out.norm;
+}
+
+Tensor clipped_sgd_step(const std::vector<Tensor>& parameters, double lr, double max_norm) {
+  at::NoGradGuard no_grad;
+  const float limit = limit_of("clipped_sgd_step", max_norm);
+  std::vector<Tensor> params, grads, packed;
+  for (const Tensor& p : parameters) {
+    const Tensor& g = p.grad();
+    if (!g.defined()) continue;
+    TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "clipped_sgd_step: a gradient must have its parameter's type, got ", g.dtype(), " for ",
+                     p.dtype());
+    params.push_back(p);
+    grads.push_back(g.layout() == at::kStrided ? dense(g) : g);
+    packed.push_back(dense(p));
+  }
+  if (params.empty()) return at::zeros({}, at::kFloat);
+  const Table t("clipped_sgd_step", grads, &packed);
+  Output out(grads[0], grads.size(), t.device);
+  check(lib.clipped_sgd(t.grads.data(), t.params.data(), t.counts.data(), t.dtypes.data(), static_cast<int64_t>(grads.size()),
+                        static_cast<float>(lr), limit, out.scratch.mutable_data_ptr<double>(), out.doubles, out.norm.mutable_data_ptr<float>(),
+                        t.device, stream_of(t.device)),
+        "b200train_clipped_sgd");
+  for (size_t i = 0; i < params.size(); ++i) {
+    if (packed[i].is_same(params[i])) params[i].unsafeGetTensorImpl()->bump_version();
+    else params[i].copy_(packed[i]);
+  }
+  return out.norm;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_train_binding, m) {
+  m.def("set_library", &set_library);
+  m.def("add_rms_norm", &add_rms_norm);
+  m.def("rms_norm", &rms_norm);
+  m.def("router_topk", &router_topk);
+  m.def("global_grad_norm", &global_grad_norm);
+  m.def("clip_grad_norm", &clip_grad_norm);
+  m.def("clipped_sgd_step", &clipped_sgd_step);
+}

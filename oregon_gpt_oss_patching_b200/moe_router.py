@@ -16,72 +16,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _cabi
+from . import _binding
 
 __all__ = ["router_topk", "b200_router_forward", "patch_moe_router", "unpatch_moe_router"]
-
-_SCORINGS = {"softmax": 0, "sigmoid": 1}
-
-
-def _check(logits, top_k, scoring, bias, num_groups, top_groups):
-    if not logits.is_cuda:
-        raise RuntimeError("router_topk needs CUDA tensors (the sm_100a library is the only code path)")
-    if logits.dtype not in _cabi.MOE_DTYPES:
-        raise TypeError(f"router_topk supports bfloat16, float16 and float32 logits, got {logits.dtype}")
-    if logits.dim() != 2:
-        raise ValueError(f"router_topk: logits must be (tokens, experts), got {tuple(logits.shape)}")
-    if scoring not in _SCORINGS:
-        raise ValueError(f"router_topk: scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
-    E = logits.shape[1]
-    if not 1 <= E <= _cabi.MOE_ROUTER_MAX_EXPERTS:
-        raise ValueError(f"router_topk: 1 to {_cabi.MOE_ROUTER_MAX_EXPERTS} experts, got {E}")
-    if not 1 <= num_groups <= _cabi.MOE_ROUTER_MAX_GROUPS or E % num_groups or not 1 <= top_groups <= num_groups:
-        raise ValueError(f"router_topk: {E} experts cannot form {num_groups} equal groups of which {top_groups} are eligible")
-    if not 1 <= top_k <= min(_cabi.MOE_ROUTER_MAX_TOP_K, E // num_groups * top_groups):
-        raise ValueError(f"router_topk: cannot choose {top_k} of {E // num_groups * top_groups} eligible experts (at most "
-                         f"{_cabi.MOE_ROUTER_MAX_TOP_K})")
-    if bias is not None and (bias.shape != (E,) or bias.device != logits.device or not bias.is_floating_point()):
-        raise ValueError(f"router_topk: bias must be {E} floating point values on {logits.device}")
-
-
-class _router_topk(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, top_k, sigmoid, num_groups, top_groups, renormalize, scale):
-        if logits.stride(1) != 1 and logits.shape[1] > 1:
-            logits = logits.contiguous()
-        T, E = logits.shape
-        if bias is not None:
-            bias = bias.to(torch.float32).contiguous()
-        weights = torch.empty((T, top_k), dtype=logits.dtype, device=logits.device)
-        indices = torch.empty((T, top_k), dtype=torch.int64, device=logits.device)
-        dev = logits.device
-        rc = _cabi.load().b200moe_router_topk(
-            logits.data_ptr(), logits.stride(0), None if bias is None else bias.data_ptr(), weights.data_ptr(), indices.data_ptr(), T, E,
-            top_k, num_groups, top_groups, sigmoid, renormalize, scale, _cabi.MOE_DTYPES[logits.dtype], dev.index,
-            torch.cuda.current_stream(dev).cuda_stream)
-        _cabi.check(rc, "b200moe_router_topk")
-        ctx.save_for_backward(logits, indices)
-        ctx.how = sigmoid, renormalize, scale
-        ctx.mark_non_differentiable(indices)
-        return weights, indices
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dweights, _):
-        logits, indices = ctx.saved_tensors
-        sigmoid, renormalize, scale = ctx.how
-        T, E = logits.shape
-        dev = logits.device
-        dweights = dweights.contiguous()
-        dlogits = torch.empty((T, E), dtype=logits.dtype, device=dev)
-        rc = _cabi.load().b200moe_router_topk_bwd(
-            logits.data_ptr(), logits.stride(0), indices.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), T, E, indices.shape[1], sigmoid,
-            renormalize, scale, _cabi.MOE_DTYPES[logits.dtype], dev.index, torch.cuda.current_stream(dev).cuda_stream)
-        _cabi.check(rc, "b200moe_router_topk_bwd")
-        return dlogits, None, None, None, None, None, None, None
-
 
 def router_topk(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, num_groups: int = 1,
                 top_groups: Optional[int] = None, renormalize: bool = True, scale: float = 1.0):
@@ -92,10 +30,7 @@ def router_topk(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", b
     for the choice alone and gets no gradient; with ``num_groups`` only the experts of the ``top_groups`` groups with the
     largest sums of their two best values are eligible; ``renormalize`` divides the weights by their sum; ``scale`` multiplies them.
     """
-    top_groups = num_groups if top_groups is None else top_groups
-    _check(logits, top_k, scoring, bias, num_groups, top_groups)
-    return _router_topk.apply(logits, None if bias is None else bias.detach(), int(top_k), _SCORINGS[scoring], int(num_groups), int(top_groups),
-                              int(bool(renormalize)), float(scale))
+    return _binding.load().router_topk(logits, top_k, scoring, bias, num_groups, num_groups if top_groups is None else top_groups, renormalize, scale)
 
 
 def b200_router_forward(self, hidden_states: torch.Tensor):
