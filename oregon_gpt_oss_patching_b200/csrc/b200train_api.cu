@@ -29,10 +29,11 @@ bool known_dtype(int dtype) { return dtype >= B200TRAIN_BF16 && dtype <= B200TRA
 
 // Launches a kernel that may start while the one before it in the stream runs out; it waits for that one's end itself.
 template <typename... P, typename... A>
-int launch_dependent(void (*kernel)(P...), unsigned grid, dim3 block, cudaStream_t st, A... args) {
+int launch_dependent(void (*kernel)(P...), unsigned grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(grid);
   config.blockDim = block;
+  config.dynamicSmemBytes = smem;
   config.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -139,9 +140,11 @@ int with_shape(const NormShape& s, F f) {
 
 // ---------------------------------------------------------------- clip
 
-constexpr int kClipCtasPerSm = 8;
-
-int clip_grid(int device) { return sm_count(device) * kClipCtasPerSm; }
+// CTAs an SM: of 3, 4, 6 and 8 the fastest on one decoder layer's gradients (within 4 % of one another).
+constexpr int kSumCtas = 6, kApplyCtas = 4;
+// Shared memory that the second kernel takes and does not use: no SM has room for a fifth CTA.  They arrive while the first
+// kernel runs out, and would crowd on the SMs that are free first (clip 882 us instead of 780).
+constexpr size_t kApplySmem = 46 * 1024;
 
 enum class ClipOp { kNorm, kClip, kSgd };
 
@@ -214,29 +217,27 @@ int run_clip(ClipOp op, const int64_t* grads, const int64_t* params, const int64
   DeviceGuard guard(device);
   if (!guard.ok) return B200ATTN_ECUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int cap = clip_grid(device);
+  const int sms = sm_count(device);
   ClipTable t;
   int parts = 0;
   for (int64_t i = 0; i < tensors;) {
     i += fill_table(&t, grads, params, counts, dtypes, i, tensors);
     if (t.tensors == 0) continue;
-    const int grid = t.chunks < (unsigned)cap ? (int)t.chunks : cap;
+    const int grid = (int)std::min<unsigned>(t.chunks, sms * kSumCtas);
     grad_sumsq_kernel<<<grid, kClipThreads, 0, st>>>(t, scratch + parts);
     parts += grid;
     if ((rc = launch_status())) return rc;
   }
-  if (op == ClipOp::kNorm || parts == 0) {
-    grad_norm_kernel<<<1, kClipThreads, 0, st>>>(scratch, parts, norm);
-    return launch_status();
-  }
+  const double* partials = scratch;
+  if (op == ClipOp::kNorm || parts == 0) return launch_dependent(grad_norm_kernel, 1, dim3(kClipThreads), 0, st, partials, parts, norm);
+  auto* apply = op == ClipOp::kSgd ? clip_apply_kernel<true> : clip_apply_kernel<false>;
   for (int64_t i = 0; i < tensors;) {
     if (tensors > kClipTensors) i += fill_table(&t, grads, params, counts, dtypes, i, tensors);
     else i = tensors;   // (the table of the first kernel serves again)
     if (t.tensors == 0) continue;
-    const int grid = t.chunks < (unsigned)cap ? (int)t.chunks : cap;
-    if (op == ClipOp::kSgd) clip_apply_kernel<true><<<grid, kClipThreads, 0, st>>>(t, scratch, parts, max_norm, lr, norm);
-    else clip_apply_kernel<false><<<grid, kClipThreads, 0, st>>>(t, scratch, parts, max_norm, 0.f, norm);
-    if ((rc = launch_status())) return rc;
+    rc = launch_dependent(apply, std::min<unsigned>(t.chunks, sms * kApplyCtas), dim3(kClipThreads), kApplySmem, st, t, partials, parts, max_norm,
+                          lr, norm);
+    if (rc) return rc;
   }
   return B200ATTN_OK;
 }
@@ -313,7 +314,7 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
       return launch_status();
     });
     if (rc2 || dweight == nullptr) return rc2;
-    return launch_dependent(norm_dw_kernel<W>, (cols + 31) / 32, dim3(32, 32), st, static_cast<const float*>(scratch), static_cast<W*>(dweight),
+    return launch_dependent(norm_dw_kernel<W>, (cols + 31) / 32, dim3(32, 32), 0, st, static_cast<const float*>(scratch), static_cast<W*>(dweight),
                             s.grid, cols);
   });
 }
@@ -321,7 +322,7 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
 // (one partial a CTA of every launch; every launch but the last takes kClipTensors tensors)
 int64_t b200train_clip_scratch_doubles(int64_t tensors, int32_t device) {
   if (tensors < 0) return 0;
-  return (tensors / kClipTensors + 1) * clip_grid(device);
+  return (tensors / kClipTensors + 1) * sm_count(device) * kSumCtas;
 }
 
 int b200train_grad_norm(const int64_t* grads, const int64_t* counts, const int32_t* dtypes, int64_t tensors, double* scratch,

@@ -6,7 +6,9 @@ the model is built from ``GptOssConfig`` with random bf16 weights (no checkpoint
 token ids are uniform over the vocabulary), attention is patched exactly as the reference does
 (``sft.py:18``), gradient checkpointing is on (``sft_full.yaml:13``), batch 1 per GPU and
 ``max_length`` 8192 (``sft_full.yaml:16,18``); the expert block runs through this library's grouped GEMMs unless
-``--moe hf`` / ``--moe hf_eager`` asks for transformers' own implementations.  Data parallelism is plain replication with a
+``--moe hf`` / ``--moe hf_eager`` asks for transformers' own implementations.  ``--norm b200`` and ``--router b200`` patch the
+RMS norms and the router as well, and ``--max-grad-norm`` clips the gradients as the reference's launcher does (1.0,
+``zero3.yaml:6``), folded into the update.  Data parallelism is plain replication with a
 bucketed NCCL all-reduce of the bf16 gradients (torch DDP) instead of DeepSpeed ZeRO-3, and the
 optimizer is state-free SGD, so that one replica (41.8 GB weights + 41.8 GB gradients for the 20b
 architecture) fits one 180 GB GPU.
@@ -67,6 +69,11 @@ def main():
                     "all-reduce (the difference to a normal run is the part of the all-reduce that backward does not hide)")
     ap.add_argument("--gemm-ctas", type=int, default=0, help="persistent CTAs of the grouped GEMM (0 = one per SM); fewer "
                     "leaves SMs to the all-reduce that runs beside the backward pass")
+    ap.add_argument("--norm", default="hf", choices=["hf", "b200"], help="RMS norms and the residual sum between attention and experts: "
+                    "transformers', or the fused kernels")
+    ap.add_argument("--router", default="hf", choices=["hf", "b200"], help="choice of experts: transformers' top-k and softmax, or the fused kernel")
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="clip the global gradient norm; the clip and the update are one "
+                    "call (default: no clipping, torch's update)")
     ap.add_argument("--hf-rope", action="store_true", help="keep transformers' rotary embedding (default: the one-pass kernel, "
                     "whenever the attention is patched)")
     args = ap.parse_args()
@@ -91,6 +98,15 @@ def main():
         moe_experts.patch_moe_experts()
         moe_experts.set_gemm_ctas(args.gemm_ctas)
 
+    if args.norm == "b200":
+        from . import rms_norm
+        rms_norm.patch_rms_norm()
+    if args.router == "b200":
+        from . import moe_router
+        moe_router.patch_moe_router()
+    if args.max_grad_norm is not None:
+        from . import grad_clip
+
     model, cfg = build_model(args.layers, args.experts, args.vocab, dev, experts_implementation="eager" if args.moe == "hf_eager" else None)
     n_params = sum(p.numel() for p in model.parameters())
     net = model
@@ -103,12 +119,16 @@ def main():
     def step():
         out = net(input_ids=ids, labels=ids, use_cache=False)
         out.loss.backward()
+        norm = None
         with torch.no_grad():
             params = [p for p in model.parameters() if p.grad is not None]
-            torch._foreach_add_(params, [p.grad for p in params], alpha=-args.lr)
+            if args.max_grad_norm is not None:
+                norm = grad_clip.clipped_sgd_step(params, args.lr, args.max_grad_norm)
+            else:
+                torch._foreach_add_(params, [p.grad for p in params], alpha=-args.lr)
             for p in params:
                 p.grad = None
-        return out.loss.detach()
+        return out.loss.detach(), norm
 
     for _ in range(args.warmup):
         step()
@@ -119,7 +139,7 @@ def main():
     e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     e0.record()
     for _ in range(args.steps):
-        loss = step()
+        loss, norm = step()
     e1.record()
     torch.cuda.synchronize(dev)
     ms = torch.tensor([e0.elapsed_time(e1) / args.steps], dtype=torch.float64, device=dev)
@@ -135,6 +155,8 @@ def main():
             "n_gpus": world, "ms_per_step": round(ms.item(), 1), "steps": args.steps, "warmup": args.warmup,
             "attention": "hf_eager" if args.unpatched else "b200",
             "rope": "hf" if (args.unpatched or args.hf_rope) else "b200",
+            "norm": args.norm, "router": args.router, "max_grad_norm": args.max_grad_norm,
+            "grad_norm": None if norm is None else round(float(norm), 4),
             "moe": args.moe if args.moe != "hf" else "hf:" + str(getattr(cfg, "_experts_implementation", None)), "loss": round(float(loss), 4), "kernel_status": status,
             "config": {"layers": args.layers, "experts": args.experts, "vocab": args.vocab, "seq_len": args.seq,
                        "params_b": round(n_params / 1e9, 2), "batch_per_gpu": 1, "gemm_ctas": args.gemm_ctas, "grad_checkpointing": True,
