@@ -71,14 +71,24 @@ bool on_grid(const void* p, int64_t stride, int run, int size) {
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0;
 }
 
+template <typename T, int RL, int RUNS, int LL>
+void launch_quick_router(const RouterArgs& a, cudaStream_t st) {
+  const int grid = (int)(((long long)a.tokens + kQuickTokens - 1) / kQuickTokens);
+  if (a.bias != nullptr || a.groups > 1) router_topk_kernel<T, RL, RUNS, LL, true><<<grid, kRouterThreads, 0, st>>>(a);
+  else router_topk_kernel<T, RL, RUNS, LL, false><<<grid, kRouterThreads, 0, st>>>(a);
+}
+// By how many experts a lane holds; a token's 8 lanes keep the best 4 or 8.
 template <typename T, int VPL>
 void launch_router(RouterArgs a, cudaStream_t st) {
-  const bool exact = sizeof(T) == 2 && a.bias == nullptr && a.groups == 1;
-  a.slow = !exact && (a.top_k >= 32 || (a.groups & (a.groups - 1)) != 0);
-  a.vector = a.experts == 32 * VPL && on_grid(a.logits, a.stride, VPL, sizeof(T));   // (every lane holds VPL neighbours)
-  const int grid = (a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32);
-  if (a.bias != nullptr || a.groups > 1) router_topk_kernel<T, VPL, true><<<grid, kRouterThreads, 0, st>>>(a);
-  else router_topk_kernel<T, VPL, false><<<grid, kRouterThreads, 0, st>>>(a);
+  if (a.top_k > 8 || a.groups > kQuickLanes || (a.groups & (a.groups - 1)) != 0) {
+    router_topk_any_kernel<T><<<(int)(((long long)a.tokens + 7) / 8), kRouterThreads, 0, st>>>(a);
+    return;
+  }
+  constexpr int RL = VPL == 1 ? 4 : 8, RUNS = VPL <= 2 ? 1 : VPL / 2;
+  a.vector = a.experts == kQuickLanes * RL * RUNS && on_grid(a.logits, a.stride, RL, sizeof(T));   // (every lane holds whole runs)
+  a.vector_bias = a.vector && on_grid(a.bias, 0, RL, sizeof(float));
+  if (a.top_k <= 4) launch_quick_router<T, RL, RUNS, 4>(a, st);
+  else launch_quick_router<T, RL, RUNS, 8>(a, st);
 }
 template <typename T, int VPL>
 void launch_router(RouterBwdArgs a, cudaStream_t st) {

@@ -8,18 +8,19 @@
 // GptOssTopKRouter.forward (transformers/models/gpt_oss/modeling_gpt_oss.py:126-133) is softmax, no bias, no groups, renormalised:
 // the softmax over the chosen logits.
 //
-// One warp serves one token.  A lane holds up to 8 experts (whole lanes to a group) as keys: the upper 24 bits of the value in
-// an order of unsigned integers, and 255 - expert below, so that keys differ and the larger one is the one to elect.  The lane
-// sorts its keys; a round of the election is one warp-wide integer maximum (`redux.sync`) of the lanes' first keys, and the lane
-// that has it moves up its list.  Instructions bound the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid,
-// bias, 4 of 8 groups take @FWD@ us forward and @BWD@ us backward.  (Full keys with two maxima a round, unsorted lists and groups
-// summed through shared memory, as the slow path below has it: 89 us.)
+// The quick election (top_k <= 8; 1, 2, 4 or 8 groups): 8 lanes serve a token, 4 tokens a warp.  A lane turns its up to 32
+// experts (whole lanes to a group) into keys: the upper 24 bits of the value in an order of unsigned integers, and 255 - expert
+// below, so that keys differ and the larger one is the one to elect.  It sorts them by eights with a network, keeps the best 8
+// (or 4, where top_k allows), and three exchanges between the lanes leave the token's best in all of them.  Instructions bound
+// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 42 us forward (28 us without the
+// doubtful tokens, below), on logits alone 15 us, and 12 us backward.  (A warp a token with a warp-wide maximum a round: 66 and 25 us; that with full keys, two
+// maxima a round and groups summed through shared memory, as the slow election below has it: 89 and 37 us.)
 //
 // 24 bits hold every bf16 and fp16 logit, so the choice is exact where neither bias nor groups take part (scores rise with
-// logits).  Otherwise lane j looks at the gap between the (j - 1)-th and the j-th value elected, one more than is wanted among
-// them, and at the border between groups.  Where a gap is not wider than what the keys and fp32 lose (and the two do not come
-// from the same logit and bias, where the lower index is right), the warp elects again, in full fp32 and, where that cannot tell
-// either, in fp64: about one token in 300 of random ones.
+// logits).  Otherwise a lane looks at the gap between its and the last lane's value, at the one behind the last elected and at
+// the border between groups.  Where a gap is not wider than what the keys and fp32 lose (and the two do not come from the
+// same logit and bias, where the lower index is right), the whole warp elects for that token again, in
+// fp64: about one token in 450 of random ones.
 #pragma once
 #include <math_constants.h>
 
@@ -32,9 +33,11 @@ using b200train::pack;
 using b200train::unpack;
 
 constexpr int kRouterThreads = 256;
-constexpr int kRouterMaxExperts = 256;   // 8 a lane
+constexpr int kRouterMaxExperts = 256;   // 8 a lane of the slow election, 32 a lane of the quick one
 constexpr int kRouterMaxTopK = 32;       // one a lane
 constexpr int kRouterMaxGroups = 32;     // one lane a group at least
+constexpr int kQuickLanes = 8;           // of a token
+constexpr int kQuickTokens = kRouterThreads / kQuickLanes;
 
 // fp32 and fp64 values as unsigned keys in the same order; NaN above everything (as torch.topk has it), -0 as 0.
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -47,33 +50,21 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
   if (v != v) return ~0ull;
   return (b >> 63) ? ~b : b | (1ull << 63);
 }
-__device__ __forceinline__ uint32_t warp_max_key(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
-__device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
-    k = other > k ? other : k;
-  }
-  return k;
+
+// Sums and maxima over runs of `width` lanes (a power of two).
+template <typename V>
+__device__ __forceinline__ V lanes_add(V v, int width) {
+  for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 template <typename V>
-__device__ __forceinline__ V warp_max(V v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+__device__ __forceinline__ V lanes_max(V v, int width) {
+  for (int o = width >> 1; o > 0; o >>= 1) {
     const V other = __shfl_xor_sync(0xffffffffu, v, o);
     v = other > v || other != other ? other : v;   // (a NaN wins)
   }
   return v;
 }
-template <typename V>
-__device__ __forceinline__ V warp_add(V v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
 struct RouterArgs {
   const void* logits;       // (tokens, experts), row stride below
@@ -83,184 +74,116 @@ struct RouterArgs {
   long long* indices;       // (tokens, top_k)
   int tokens, experts, top_k, groups, top_groups;
   int sigmoid, renormalize;
-  int vector;               // a lane's experts can be loaded at once
-  int slow;                 // top_k or the groups are beyond the quick election
+  int vector, vector_bias;  // a lane's experts, their biases can be loaded at once
   float scale;
 };
 
-// The scores of this lane's experts, in V's precision.
-template <typename V, int VPL>
-__device__ __forceinline__ void scores_of(const float (&l)[VPL], bool sigmoid, V (&s)[VPL]) {
-  if (sigmoid) {
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) s[i] = V(1) / (V(1) + exp_of(-V(l[i])));
-  } else {
-    float m = l[0];
-#pragma unroll
-    for (int i = 1; i < VPL; ++i) m = l[i] > m || l[i] != l[i] ? l[i] : m;
-    m = warp_max(m);
-    V z = 0;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      s[i] = l[i] == -CUDART_INF_F ? V(0) : exp_of(V(l[i]) - V(m));
-      z += s[i];
+// The slow election: any groups and top_k, values in fp64, a whole warp a token; lane j's return is the j-th expert.  `row` (shared,
+// of this warp) holds the values by expert, later their keys.  Loops instead of registers keep the code small: it is cold when a
+// doubtful token of the quick election comes to it, and instruction fetches are what it waits for (the same unrolled over
+// registers, with an fp32 try first, took the kernel 48 us instead of 42).
+template <typename T>
+__device__ __noinline__ int elect_slowly(const RouterArgs& a, const T* logits, int lane, unsigned long long* row) {
+  const bool by_logit = a.bias == nullptr && a.groups == 1;   // scores rise with logits
+  double m = 0.0, z = 1.0;
+  if (!a.sigmoid && !by_logit) {
+    float top = -CUDART_INF_F;
+    for (int e = lane; e < a.experts; e += 32) {
+      const float l = Elem<T>::load1(logits + e);
+      top = l > top || l != l ? l : top;
     }
-    z = warp_add(z);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) s[i] = z == V(0) ? V(0) : s[i] / z;
+    m = lanes_max(top, 32);
   }
-}
-
-template <typename V>
-struct Top2 {
-  V first, second;
-  __device__ __forceinline__ void add(V v) {
-    if (v > first || v != v) { second = first; first = v; }
-    else if (v > second) second = v;
-  }
-  __device__ __forceinline__ V sum() const { return second > V(-CUDART_INF_F) ? first + second : first; }
-};
-
-// Which groups stand for election, as a bit mask.  `row` (shared, of this warp) holds the values by expert.  The lanes are
-// shared out: `part` of them (a power of two) walk one group.  `close` is set where the border between the groups chosen
-// and those left is narrower than `margin` (times 1 + the value).
-template <typename V>
-__device__ __forceinline__ uint32_t open_groups(const V* row, const RouterArgs& a, int lane, V margin, bool& close) {
-  int part = 32;
-  while (part * a.groups > 32) part >>= 1;
-  const int size = a.experts / a.groups, g = lane / part, p = lane % part;
-  Top2<V> best{V(-CUDART_INF_F), V(-CUDART_INF_F)};
-  if (g < a.groups)
-    for (int j = p; j < size; j += part) best.add(row[g * size + j]);
-  for (int o = part >> 1; o > 0; o >>= 1) {
-    const V f = __shfl_xor_sync(0xffffffffu, best.first, o), s = __shfl_xor_sync(0xffffffffu, best.second, o);
-    best.add(f);
-    best.add(s);
-  }
-  // lane g now ranks group g among all
-  const V sums = best.sum();
-  const V mine = __shfl_sync(0xffffffffu, sums, (lane * part) & 31);
-  const auto key = order_key(mine);
-  int ahead = 0;
-  for (int other = 0; other < a.groups; ++other) {
-    const auto k = __shfl_sync(0xffffffffu, key, other);
-    ahead += k > key || (k == key && other < lane);
-  }
-  const bool chosen = lane < a.groups && ahead < a.top_groups;
-  const uint32_t mask = __ballot_sync(0xffffffffu, chosen);
-  if (margin > V(0) && a.top_groups < a.groups) {
-    const uint32_t last_in = __ballot_sync(0xffffffffu, lane < a.groups && ahead == a.top_groups - 1);
-    const uint32_t first_out = __ballot_sync(0xffffffffu, lane < a.groups && ahead == a.top_groups);
-    const V in = __shfl_sync(0xffffffffu, mine, __ffs(last_in) - 1), out = __shfl_sync(0xffffffffu, mine, __ffs(first_out) - 1);
-    // (two groups without an expert that is not masked are a true tie)
-    close = !(in - out > margin * (V(1) + fabs(in))) && !(in == V(-CUDART_INF_F) && out == V(-CUDART_INF_F));
-  }
-  return mask;
-}
-
-// An election's outcome: lane j (< top_k) holds the j-th expert and its logit.
-struct Elected {
-  int expert;
-  float logit;
-};
-
-// V: float or double values (kValues), or the logits themselves (!kValues).
-template <typename V, int VPL, bool kValues>
-__device__ __forceinline__ Elected elect(const float (&l)[VPL], const float (&b)[VPL], const RouterArgs& a, int lane, V* row, bool check, bool& close) {
-  using Key = decltype(order_key(V(0)));
-  Key key[VPL];
-  close = false;
-  if constexpr (kValues) {
-    V v[VPL];
-    scores_of<V, VPL>(l, a.sigmoid != 0, v);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) v[i] = l[i] == -CUDART_INF_F ? V(-CUDART_INF_F) : v[i] + V(b[i]);
-    uint32_t open = 0xffffffffu;
-    if (a.groups > 1) {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (lane + 32 * i < a.experts) row[lane + 32 * i] = v[i];
-      __syncwarp();
-      open = open_groups<V>(row, a, lane, check ? V(8e-6) : V(0), close);
-      __syncwarp();
-    }
-    const int size = a.experts / a.groups;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = lane + 32 * i;
-      key[i] = e < a.experts && (a.groups == 1 || (open >> (e / size)) & 1u) ? order_key(v[i]) : Key(0);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) key[i] = lane + 32 * i < a.experts ? order_key(V(l[i])) : Key(0);
-  }
-  Elected out{0, 0.f};
-  float last_l = 0.f, last_b = 0.f;
-  V last_v = 0;
-  // one round more than is elected, to see the gap behind the last one
-  const int rounds = kValues && check && a.top_k < a.experts ? a.top_k + 1 : a.top_k;
-  for (int j = 0; j < rounds; ++j) {
-    Key best = key[0];
-    int at = 0;
-#pragma unroll
-    for (int i = 1; i < VPL; ++i)
-      if (key[i] > best) { best = key[i]; at = i; }
-    const Key top = warp_max_key(best);
-    if (kValues && top == Key(0)) break;   // (no expert is left behind the last one elected)
-    const int e = (int)__reduce_min_sync(0xffffffffu, best == top ? (uint32_t)(lane + 32 * at) : 0xffffffffu);
-    const int slot = e >> 5, owner = e & 31;
-    float le = 0.f, be = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (i == slot) {
-        le = l[i];
-        be = b[i];
-        if (lane == owner) key[i] = Key(0);
+  // the first turn sums the softmax, the second writes the values
+  for (int turn = a.sigmoid || by_logit ? 1 : 0; turn < 2; ++turn) {
+    double sum = 0.0;
+#pragma unroll 1
+    for (int e = lane; e < a.experts; e += 32) {
+      const float l = Elem<T>::load1(logits + e);
+      double v = l;
+      if (!by_logit && l != -CUDART_INF_F) {
+        const double x = exp(a.sigmoid ? -v : v - m);
+        sum += x;
+        v = (a.sigmoid ? 1.0 : x) / (a.sigmoid ? 1.0 + x : z) + (a.bias != nullptr ? (double)a.bias[e] : 0.0);
       }
-    le = __shfl_sync(0xffffffffu, le, owner);
-    if constexpr (kValues) {
-      if (check) {
-        be = __shfl_sync(0xffffffffu, be, owner);
-        // the value back from its key
-        const uint32_t bits = (top & 0x80000000u) ? (uint32_t)top & 0x7fffffffu : ~(uint32_t)top;
-        const V v = V(__uint_as_float(bits));
-        const bool same = __float_as_uint(le) == __float_as_uint(last_l) && (be == last_b || le == -CUDART_INF_F);
-        if (j > 0 && !same && !(last_v - v > V(4e-6) * (V(1) + fabs(v)))) close = true;
-        last_l = le;
-        last_b = be;
-        last_v = v;
+      row[e] = (unsigned long long)__double_as_longlong(v);
+    }
+    if (turn == 0) z = lanes_add(sum, 32);
+  }
+  __syncwarp();
+  uint32_t open = 0xffffffffu;
+  const int size = a.experts / a.groups;
+  if (a.groups > 1) {
+    int part = 32;   // lanes that look through one group
+    while (part * a.groups > 32) part >>= 1;
+    double best = -CUDART_INF, next = -CUDART_INF;
+    bool number = true;
+    if (lane / part < a.groups) {
+      for (int i = lane % part; i < size; i += part) {
+        const double v = __longlong_as_double((long long)row[lane / part * size + i]);
+        number = number && v == v;
+        next = fmax(next, fmin(best, v));
+        best = fmax(best, v);
       }
     }
-    if (lane == j) out = Elected{e, le};
+    for (int o = part >> 1; o > 0; o >>= 1) {
+      const double f = __shfl_xor_sync(0xffffffffu, best, o), n = __shfl_xor_sync(0xffffffffu, next, o);
+      next = fmax(fmin(best, f), fmax(next, n));
+      best = fmax(best, f);
+      number = __shfl_xor_sync(0xffffffffu, (int)number, o) && number;
+    }
+    double sum = !number ? CUDART_NAN : next == -CUDART_INF ? best : best + next;
+    sum = __shfl_sync(0xffffffffu, sum, lane * part & 31);   // lane g ranks group g
+    const unsigned long long key = order_key(sum);
+    int ahead = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const unsigned long long other = __shfl_sync(0xffffffffu, key, g);
+      ahead += other > key || (other == key && g < lane);
+    }
+    open = __ballot_sync(0xffffffffu, lane < a.groups && ahead < a.top_groups);
+    __syncwarp();
   }
-  return out;
+  // keys: 0 for an expert of a closed group and for one elected already
+#pragma unroll 1
+  for (int e = lane; e < a.experts; e += 32)
+    row[e] = a.groups == 1 || (open >> (e / size) & 1u) ? order_key(__longlong_as_double((long long)row[e])) : 0ull;
+  int elected = 0;
+#pragma unroll 1
+  for (int j = 0; j < a.top_k; ++j) {
+    unsigned long long best = 0ull;
+    int at = a.experts;
+#pragma unroll 2
+    for (int e = lane; e < a.experts; e += 32) {   // (the lane's own entries: no other lane writes them)
+      const unsigned long long k = row[e];
+      if (k > best) {
+        best = k;
+        at = e;
+      }
+    }
+    // the largest upper half, of those the largest lower half, of those the lowest expert
+    const uint32_t upper = (uint32_t)(best >> 32), lower = (uint32_t)best;
+    const bool ahead = upper == __reduce_max_sync(0xffffffffu, upper);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, ahead ? lower : 0u);
+    const int winner = (int)__reduce_min_sync(0xffffffffu, ahead && lower == top ? (uint32_t)at : 0xffffffffu);
+    if (lane == (winner & 31)) row[winner] = 0ull;
+    if (lane == j) elected = winner;
+  }
+  __syncwarp();
+  return elected;
 }
 
-// The election in full precision, for any groups and top_k: lane j's return is the j-th expert.  `row` is shared memory of this warp.
-template <typename T, int VPL>
-__device__ __noinline__ int elect_slowly(const RouterArgs& a, const T* logits, int lane, double* row) {
-  float l[VPL], b[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    const int e = lane + 32 * i;
-    l[i] = e < a.experts ? Elem<T>::load1(logits + e) : -CUDART_INF_F;
-    b[i] = a.bias != nullptr && e < a.experts ? a.bias[e] : 0.f;
-  }
-  bool close;
-  if (a.bias == nullptr && a.groups == 1) return elect<float, VPL, false>(l, b, a, lane, nullptr, false, close).expert;
-  const int e = elect<float, VPL, true>(l, b, a, lane, reinterpret_cast<float*>(row), true, close).expert;
-  if (!close) return e;   // (the same in every lane)
-  return elect<double, VPL, true>(l, b, a, lane, row, false, close).expert;
-}
-
-constexpr float kKeyStep = 2.f / 32768.f;   // two steps of a key's 15 bits of mantissa, relative
-constexpr float kValueError = 4e-6f;        // of two values of 1 + |v|, with their scores' errors
+// How far the difference of two values of the quick election may be from the true one, over 1 + |v|.  u = 2^-24.
+//   sigmoid   __expf is right to (2 + 1.17 |l|) 2 u, of which s (1 - s) arrives: 1.2 u at most; 1 + e, 2 ulp of the quotient and the
+//             sum with the bias: 1, 2 and |v| u.  Twice that: below 9 u + 2 u |v|.
+//   softmax   expf, its argument and the quotient: below 5 u of s; the sum of 32 terms a lane and three exchanges: 37 u of s; the two
+//             scores are at most 1 together: 42 u + 2 u |v|.
+__device__ __forceinline__ float value_error(bool sigmoid) { return sigmoid ? 10.f / 16777216.f : 48.f / 16777216.f; }
 
 __device__ __forceinline__ uint32_t make_key(float v, int expert) { return (order_key(v) & 0xffffff00u) | (255u - expert); }
-// the middle of the values that share a key's upper 24 bits; -inf for a masked expert's
-__device__ __forceinline__ float key_value(uint32_t key) {
+// the largest of the values that share a key's upper 24 bits; -inf for a masked expert's
+__device__ __forceinline__ float key_ceiling(uint32_t key) {
   if (key <= 0x007fffffu) return -CUDART_INF_F;
-  const uint32_t u = (key & 0xffffff00u) | 0x80u;
+  const uint32_t u = key | 0xffu;
   return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ void sort_pair(uint32_t& a, uint32_t& b) {
@@ -346,121 +269,213 @@ __device__ __forceinline__ void store_run(T* p, int n, bool vector, const float 
 // A score fit to be elected by: expf and a true quotient cost three times as much and tell no more apart.
 __device__ __forceinline__ float quick_sigmoid(float l) { return __fdividef(1.f, 1.f + __expf(-l)); }
 
-// kValues: a bias or groups take part.  The host sees to it that a group has whole lanes (their number a power of two) and
-// top_k < 32, or asks for the slow path at once.
-template <typename T, int VPL, bool kValues>
-__global__ void __launch_bounds__(kRouterThreads) router_topk_kernel(const __grid_constant__ RouterArgs a) {
-  constexpr bool kExact = !kValues && sizeof(T) == 2;
-  __shared__ double rows[kValues ? kRouterThreads / 32 : 1][kValues ? 32 * VPL : 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = blockIdx.x * (kRouterThreads / 32) + warp;
-  if (t >= a.tokens) return;
-  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
-  float l[VPL], m = 0.f, z = 1.f;
-  uint32_t key[VPL];
-  const int groups = a.slow ? 1 : a.groups, part = 32 / groups, size = a.experts / groups, per = (size + part - 1) / part;   // lanes a group, experts a group, a lane
-  const int group = lane / part, place = lane % part * per;
-  const int first = group * size + place, mine = max(0, min(per, size - place));
-  load_run<T, VPL>(row + first, mine, a.vector != 0, l);
-  if (!a.sigmoid && (kValues || !a.renormalize)) {   // the softmax's maximum and sum
-    m = l[0];
+// Keeps the best LL of two falling lists in `a`, in falling order; `lost` is the largest key left out so far.
+template <int LL, bool kTrack>
+__device__ __forceinline__ void merge_keys(uint32_t (&a)[LL], const uint32_t (&b)[LL], uint32_t& lost) {
 #pragma unroll
-    for (int i = 1; i < VPL; ++i) m = l[i] > m || l[i] != l[i] ? l[i] : m;
-    m = warp_max(m);
-    z = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) z += l[i] == -CUDART_INF_F ? 0.f : expf(l[i] - m);
-    z = warp_add(z);
+  for (int i = 0; i < LL; ++i) {
+    if (kTrack) lost = max(lost, min(a[i], b[LL - 1 - i]));
+    a[i] = max(a[i], b[LL - 1 - i]);
   }
-  auto value = [&](float x, int e) -> float {
-    if (!kValues) return x;
-    if (x == -CUDART_INF_F) return x;
-    const float s = a.sigmoid ? quick_sigmoid(x) : __fdividef(expf(x - m), z);
-    return a.bias != nullptr ? s + a.bias[e] : s;
-  };
-  uint32_t won = 0;   // lane j's: the j-th key
-  bool sure = !a.slow;
-  if (sure) {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) key[i] = i < mine ? make_key(value(l[i], first + i), first + i) : 0u;
-    sort_keys<VPL>(key);
-    if (kValues && a.groups > 1) {
-      float best = key_value(key[0]), next = VPL > 1 ? key_value(key[VPL > 1 ? 1 : 0]) : -CUDART_INF_F;
-      for (int o = part >> 1; o > 0; o >>= 1) {
-        const float f = __shfl_xor_sync(0xffffffffu, best, o), s = __shfl_xor_sync(0xffffffffu, next, o);
-        next = fmaxf(fminf(best, f), fmaxf(next, s));
-        best = fmaxf(best, f);
-      }
-      const float sum = next == -CUDART_INF_F ? best : best + next;
-      const float slack = best == -CUDART_INF_F ? 0.f : kKeyStep * (fabsf(best) + (next == -CUDART_INF_F ? 0.f : fabsf(next))) + 2.f * kValueError;
-      int ahead = 0;
-      for (int g = 0; g < a.groups; ++g) {
-        const float other = __shfl_sync(0xffffffffu, sum, g * part);
-        ahead += other > sum || (other == sum && g < group);
-      }
-      const bool open = ahead < a.top_groups;
-      // the narrowest of the gaps between an open group and a closed one
-      if (a.top_groups < a.groups) {
-        const float in = warp_max(open ? -sum : -CUDART_INF_F), out = warp_max(open ? -CUDART_INF_F : sum);
-        const float most = warp_max(slack);
-        sure = -in - out > 2.f * most || (-in == -CUDART_INF_F && out == -CUDART_INF_F);
-        sure = sure && key[0] < 0xffffff00u;   // (no NaN)
-        sure = __all_sync(0xffffffffu, sure);
-      }
+  for (int step = LL / 2; step > 0; step >>= 1) {   // (what is left rises and falls once)
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) key[i] = open ? key[i] : 0u;
-    }
-    const int rounds = kExact ? a.top_k : a.top_k + 1;
-    for (int j = 0; j < rounds; ++j) {
-      const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
-      if (lane == j) won = top;
-      const bool pop = key[0] == top;
-#pragma unroll
-      for (int i = 0; i + 1 < VPL; ++i) key[i] = pop ? key[i + 1] : key[i];
-      key[VPL - 1] = pop ? 0u : key[VPL - 1];
-    }
+    for (int i = 0; i < LL; ++i)
+      if ((i & step) == 0) sort_pair(a[i], a[i + step]);
   }
-  int expert = 255 - (int)(won & 255u);
-  const bool chosen = lane < a.top_k;
-  float x = -CUDART_INF_F;
-  if (!a.slow && (chosen || (!kExact && lane == a.top_k && won != 0u))) x = Elem<T>::load1(row + expert);
-  if (!kExact) {
-    if (!a.slow) {
-      float b = 0.f, v = x;
-      if (kValues && lane <= a.top_k && won != 0u) {
-        v = value(x, expert);
-        b = a.bias != nullptr ? a.bias[expert] : 0.f;
-      }
-      const float pv = __shfl_up_sync(0xffffffffu, v, 1), px = __shfl_up_sync(0xffffffffu, x, 1), pb = __shfl_up_sync(0xffffffffu, b, 1);
-      const bool masked = x == -CUDART_INF_F && px == -CUDART_INF_F;
-      const float gap = pv - v, error = kValues ? kValueError * (1.f + fabsf(v)) : 0.f;
-      bool fine = true;
-      if (lane > 0 && lane < a.top_k) fine = masked || (px == x && pb == b) || gap > error;
-      else if (lane == a.top_k) fine = won == 0u || masked || gap > error + kKeyStep * fabsf(pv);
-      sure = __all_sync(0xffffffffu, fine) && sure;
-    }
-    if (!sure) {   // (the same in every lane)
-      expert = elect_slowly<T, VPL>(a, row, lane, rows[kValues ? warp : 0]);
-      x = chosen ? Elem<T>::load1(row + expert) : -CUDART_INF_F;
-    }
-  }
-  // the weights of the elected
+}
+
+// The weights of the elected: lane j (of `width` that serve the token) has the j-th expert and its logit x, `chosen` for
+// j < top_k.  m and z: the maximum and the sum of the softmax over all experts (not needed where it is renormalised).
+template <typename T>
+__device__ __forceinline__ void write_choice(const RouterArgs& a, long long at, bool chosen, int width, int expert, float x, float m, float z) {
   float s;
   if (a.sigmoid) {
     s = chosen ? 1.f / (1.f + expf(-x)) : 0.f;
   } else {
-    if (a.renormalize) m = warp_max(chosen ? x : -CUDART_INF_F);
+    if (a.renormalize) m = lanes_max(chosen ? x : -CUDART_INF_F, width);
     s = chosen && x != -CUDART_INF_F ? expf(x - m) : 0.f;
     if (!a.renormalize) s = z == 0.f ? 0.f : s / z;
   }
   if (a.renormalize) {
-    const float sum = warp_add(s);
+    const float sum = lanes_add(s, width);
     s = sum == 0.f ? 0.f : s / sum;
   }
   if (chosen) {
-    Elem<T>::store1(static_cast<T*>(a.weights) + (long long)t * a.top_k + lane, s * a.scale);
-    a.indices[(long long)t * a.top_k + lane] = expert;
+    Elem<T>::store1(static_cast<T*>(a.weights) + at, s * a.scale);
+    a.indices[at] = expert;
   }
+}
+
+// The quick election.  A lane holds RUNS runs of RL experts and a list of LL keys (top_k <= LL).  kValues: a bias or groups take part.
+template <typename T, int RL, int RUNS, int LL, bool kValues>
+__global__ void __launch_bounds__(kRouterThreads, 4) router_topk_kernel(const __grid_constant__ RouterArgs a) {
+  constexpr bool kExact = !kValues && sizeof(T) == 2;
+  __shared__ unsigned long long rows[kExact ? 1 : kRouterThreads / 32][kExact ? 1 : kQuickLanes * RL * RUNS];
+  const int lane = threadIdx.x & 31, place = lane % kQuickLanes, warp = threadIdx.x >> 5;
+  const long long warp_token = (long long)blockIdx.x * kQuickTokens + warp * (32 / kQuickLanes);
+  if (warp_token >= a.tokens) return;   // (whole warps leave: the lanes of a token that is not there go along)
+  const long long t = warp_token + lane / kQuickLanes;
+  const bool there = t < a.tokens;
+  const T* row = static_cast<const T*>(a.logits) + (there ? t : warp_token) * a.stride;
+  const int part = kQuickLanes / a.groups, size = a.experts / a.groups, per = (size + part - 1) / part;   // lanes a group, experts a group, a lane
+  const int group = place / part, begin = place % part * per;
+  const int first = group * size + begin, mine = max(0, min(per, size - begin));
+  float l[RUNS][RL];
+#pragma unroll
+  for (int r = 0; r < RUNS; ++r) load_run<T, RL>(row + first + r * RL, mine - r * RL, a.vector != 0, l[r]);
+  float m = 0.f, z = 1.f;
+  if (!a.sigmoid && (kValues || !a.renormalize)) {   // the softmax's maximum and sum
+    m = l[0][0];
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+      for (int i = 0; i < RL; ++i) m = l[r][i] > m || l[r][i] != l[r][i] ? l[r][i] : m;
+    m = lanes_max(m, kQuickLanes);
+    z = 0.f;
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+      for (int i = 0; i < RL; ++i) z += l[r][i] == -CUDART_INF_F ? 0.f : expf(l[r][i] - m);
+    z = lanes_add(z, kQuickLanes);
+  }
+  auto value = [&](float x, float b) -> float {
+    if (!kValues || x == -CUDART_INF_F) return x;
+    return (a.sigmoid ? quick_sigmoid(x) : __fdividef(expf(x - m), z)) + b;
+  };
+  const bool grouped = kValues && a.groups > 1;
+  float best_v = -CUDART_INF_F, next_v = -CUDART_INF_F;   // the two largest values of this lane's part of a group
+  bool numbers = true;                                    // none of them is NaN
+  uint32_t list[LL], lost = 0u;
+#pragma unroll
+  for (int i = 0; i < LL; ++i) list[i] = 0u;
+#pragma unroll
+  for (int r = 0; r < RUNS; ++r) {
+    uint32_t key[RL], best[LL];
+    float bias[RL];
+#pragma unroll
+    for (int i = 0; i < RL; ++i) bias[i] = 0.f;
+    if (kValues && a.bias != nullptr) load_run<float, RL>(a.bias + first + r * RL, mine - r * RL, a.vector_bias != 0, bias);
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+      const int e = first + r * RL + i;
+      const bool has = r * RL + i < mine;
+      const float v = has ? value(l[r][i], bias[i]) : -CUDART_INF_F;
+      key[i] = has ? make_key(v, e) : 0u;
+      if (grouped) {
+        next_v = fmaxf(next_v, fminf(best_v, v));
+        best_v = fmaxf(best_v, v);
+        numbers = numbers && v == v;
+      }
+    }
+    sort_keys<RL>(key);
+#pragma unroll
+    for (int i = 0; i < LL; ++i) best[i] = i < RL ? key[i] : 0u;
+    if (RL > LL && !kExact) lost = max(lost, key[LL < RL ? LL : 0]);
+    if (r == 0) {
+#pragma unroll
+      for (int i = 0; i < LL; ++i) list[i] = best[i];
+    } else {
+      merge_keys<LL, !kExact>(list, best, lost);
+    }
+  }
+  bool sure = true;
+  if (grouped) {
+    for (int o = part >> 1; o > 0; o >>= 1) {
+      const float f = __shfl_xor_sync(0xffffffffu, best_v, o), n = __shfl_xor_sync(0xffffffffu, next_v, o);
+      next_v = fmaxf(fminf(best_v, f), fmaxf(next_v, n));
+      best_v = fmaxf(best_v, f);
+    }
+    const float sum = next_v == -CUDART_INF_F ? best_v : best_v + next_v;
+    const float slack = best_v == -CUDART_INF_F ? 0.f : value_error(a.sigmoid) * (2.f + fabsf(best_v) + (next_v == -CUDART_INF_F ? 0.f : fabsf(next_v)));
+    int ahead = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const float other = __shfl_sync(0xffffffffu, sum, g * part, kQuickLanes);
+      ahead += other > sum || (other == sum && g < group);
+    }
+    const bool open = ahead < a.top_groups;
+    if (a.top_groups < a.groups) {   // the narrowest of the gaps between an open group and a closed one
+      const float in = -lanes_max(open ? -sum : -CUDART_INF_F, kQuickLanes), out = lanes_max(open ? -CUDART_INF_F : sum, kQuickLanes);
+      const float most = lanes_max(slack, kQuickLanes);
+      sure = (in - out > most || (in == -CUDART_INF_F && out == -CUDART_INF_F)) && numbers;
+    }
+    if (!open) {
+#pragma unroll
+      for (int i = 0; i < LL; ++i) list[i] = 0u;
+      lost = 0u;
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < kQuickLanes; o <<= 1) {
+    uint32_t other[LL];
+#pragma unroll
+    for (int i = 0; i < LL; ++i) other[i] = __shfl_xor_sync(0xffffffffu, list[i], o);
+    if (!kExact) lost = max(lost, __shfl_xor_sync(0xffffffffu, lost, o));
+    merge_keys<LL, !kExact>(list, other, lost);
+  }
+  uint32_t won = 0u;   // this lane's of the elected
+#pragma unroll
+  for (int i = 0; i < LL; ++i)
+    if (place == i) won = list[i];
+  const bool chosen = there && place < a.top_k;
+  int expert = 255 - (int)(won & 255u);
+  float x = chosen ? Elem<T>::load1(row + expert) : -CUDART_INF_F;
+  if (!kExact) {
+    float b = 0.f, v = x;
+    if (kValues && chosen) {
+      b = a.bias != nullptr ? a.bias[expert] : 0.f;
+      v = value(x, b);
+    }
+    const float pv = __shfl_up_sync(0xffffffffu, v, 1, kQuickLanes), px = __shfl_up_sync(0xffffffffu, x, 1, kQuickLanes);
+    const float pb = __shfl_up_sync(0xffffffffu, b, 1, kQuickLanes);
+    const float error = kValues ? value_error(a.sigmoid) * (1.f + fabsf(v)) : 0.f;
+    if (place > 0 && chosen) sure = sure && ((x == -CUDART_INF_F && px == -CUDART_INF_F) || (px == x && pb == b) || pv - v > error);
+    if (place == a.top_k - 1) {   // the best of those left out: no one's value is above its key's
+      uint32_t behind = lost;
+#pragma unroll
+      for (int i = 1; i < LL; ++i)
+        if (a.top_k == i) behind = list[i];
+      const float next = key_ceiling(behind);
+      sure = sure && (behind == 0u || (v == -CUDART_INF_F && next == -CUDART_INF_F) || v - next > error);
+    }
+    const uint32_t doubtful = __ballot_sync(0xffffffffu, there && !sure);
+    for (int q = 0; q < 32 / kQuickLanes; ++q) {
+      if ((doubtful >> (q * kQuickLanes) & 0xffu) == 0u) continue;
+      const T* other = static_cast<const T*>(a.logits) + (warp_token + q) * a.stride;
+      const int found = __shfl_sync(0xffffffffu, elect_slowly<T>(a, other, lane, rows[warp]), place);
+      if (lane / kQuickLanes == q) expert = found;
+      if (lane / kQuickLanes == q && chosen) x = Elem<T>::load1(row + expert);
+    }
+  }
+  write_choice<T>(a, t * a.top_k + place, chosen, kQuickLanes, expert, x, m, z);
+}
+
+// Any groups and top_k: one warp a token, the slow election.
+template <typename T>
+__global__ void __launch_bounds__(kRouterThreads) router_topk_any_kernel(const __grid_constant__ RouterArgs a) {
+  __shared__ unsigned long long rows[kRouterThreads / 32][kRouterMaxExperts];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long t = (long long)blockIdx.x * (kRouterThreads / 32) + warp;
+  if (t >= a.tokens) return;
+  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
+  float m = 0.f, z = 1.f;
+  if (!a.sigmoid && !a.renormalize) {
+    m = -CUDART_INF_F;
+    for (int e = lane; e < a.experts; e += 32) {
+      const float l = Elem<T>::load1(row + e);
+      m = l > m || l != l ? l : m;
+    }
+    m = lanes_max(m, 32);
+    z = 0.f;
+    for (int e = lane; e < a.experts; e += 32) {
+      const float l = Elem<T>::load1(row + e);
+      z += l == -CUDART_INF_F ? 0.f : expf(l - m);
+    }
+    z = lanes_add(z, 32);
+  }
+  const int expert = elect_slowly<T>(a, row, lane, rows[warp]);
+  const bool chosen = lane < a.top_k;
+  write_choice<T>(a, t * a.top_k + lane, chosen, 32, expert, chosen ? Elem<T>::load1(row + expert) : -CUDART_INF_F, m, z);
 }
 
 struct RouterBwdArgs {
@@ -500,32 +515,32 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_bwd_kernel(const _
     const float x = expf(-fabsf(lj)), s = (lj >= 0.f ? 1.f : x) / (1.f + x);   // (no overflow on either side)
     const float slope = x / ((1.f + x) * (1.f + x));
     if (a.renormalize) {
-      const float sum = warp_add(e >= 0 ? s : 0.f);
-      const float dot = warp_add(e >= 0 ? d * s : 0.f);
+      const float sum = lanes_add(e >= 0 ? s : 0.f, 32);
+      const float dot = lanes_add(e >= 0 ? d * s : 0.f, 32);
       d = sum == 0.f ? 0.f : (d - dot / sum) / sum;
     }
     chosen = d * slope;
   } else if (a.renormalize) {
-    const float m = warp_max(lj);
+    const float m = lanes_max(lj, 32);
     const float s = lj == -CUDART_INF_F ? 0.f : expf(lj - m);
-    const float sum = warp_add(s);
+    const float sum = lanes_add(s, 32);
     const float r = sum == 0.f ? 0.f : s / sum;
-    chosen = r * (d - warp_add(e >= 0 ? d * r : 0.f));
+    chosen = r * (d - lanes_add(e >= 0 ? d * r : 0.f, 32));
   } else {
     float l[VPL], z = 0.f;
     load_run<T, VPL>(row + first, n, a.vector_in != 0 && n == VPL, l);
     float m = l[0];
 #pragma unroll
     for (int i = 1; i < VPL; ++i) m = l[i] > m || l[i] != l[i] ? l[i] : m;
-    m = warp_max(m);
+    m = lanes_max(m, 32);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       g[i] = l[i] == -CUDART_INF_F ? 0.f : expf(l[i] - m);
       z += g[i];
     }
-    z = warp_add(z);
+    z = lanes_add(z, 32);
     const float s = lj == -CUDART_INF_F || z == 0.f ? 0.f : expf(lj - m) / z;
-    const float dot = warp_add(e >= 0 ? d * s : 0.f);
+    const float dot = lanes_add(e >= 0 ? d * s : 0.f, 32);
     chosen = s * (d - dot);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) g[i] = z == 0.f ? 0.f : -(g[i] / z) * dot;
