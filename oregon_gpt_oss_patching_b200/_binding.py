@@ -8,6 +8,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import threading
 
 import torch  # noqa: F401  (the module links against torch's libraries, which this import loads)
 
@@ -15,6 +16,7 @@ from . import _cabi
 from . import build as _build
 
 _NAMES = ("b200attn_strerror", "b200moe_router_topk", "b200moe_router_topk_bwd", *_cabi.TRAIN_EXPORTS)
+_lock = threading.Lock()
 _module = None
 
 
@@ -23,7 +25,8 @@ def load():
     global _module
     if _module is not None:
         return _module
-    with _cabi._lock:
+    lib = _cabi.load()
+    with _lock:
         if _module is not None:
             return _module
         if not os.path.exists(_build.BINDING_PATH):
@@ -32,7 +35,6 @@ def load():
         loader = importlib.machinery.ExtensionFileLoader("_train_binding", _build.BINDING_PATH)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_train_binding", loader))
         loader.exec_module(module)
-    lib = _cabi.load()
-    module.set_library({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _NAMES})
-    _module = module
-    return module
+        module.set_library({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _NAMES})
+        _module = module
+    return _module

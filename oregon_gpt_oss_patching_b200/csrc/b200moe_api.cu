@@ -81,7 +81,8 @@ void launch_quick_router(const RouterArgs& a, cudaStream_t st) {
 template <typename T, int VPL>
 void launch_router(RouterArgs a, cudaStream_t st) {
   if (a.top_k > 8 || a.groups > kQuickLanes || (a.groups & (a.groups - 1)) != 0) {
-    router_topk_any_kernel<T><<<(int)(((long long)a.tokens + 7) / 8), kRouterThreads, 0, st>>>(a);
+    const int grid = (int)(((long long)a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32));
+    router_topk_any_kernel<T><<<grid, kRouterThreads, 0, st>>>(a);
     return;
   }
   constexpr int RL = VPL == 1 ? 4 : 8, RUNS = VPL <= 2 ? 1 : VPL / 2;
@@ -94,7 +95,8 @@ template <typename T, int VPL>
 void launch_router(RouterBwdArgs a, cudaStream_t st) {
   a.vector_in = on_grid(a.logits, a.stride, VPL, sizeof(T));
   a.vector_out = on_grid(a.dlogits, a.experts, VPL, sizeof(T));
-  router_topk_bwd_kernel<T, VPL><<<(a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32), kRouterThreads, 0, st>>>(a);
+  const int grid = (int)(((long long)a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32));
+  router_topk_bwd_kernel<T, VPL><<<grid, kRouterThreads, 0, st>>>(a);
 }
 // by how many experts a lane holds
 template <typename T, typename Args>

@@ -12,15 +12,15 @@
 // experts (whole lanes to a group) into keys: the upper 24 bits of the value in an order of unsigned integers, and 255 - expert
 // below, so that keys differ and the larger one is the one to elect.  It sorts them by eights with a network, keeps the best 8
 // (or 4, where top_k allows), and three exchanges between the lanes leave the token's best in all of them.  Instructions bound
-// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 42 us forward (28 us without the
-// doubtful tokens, below), on logits alone 15 us, and 12 us backward.  (A warp a token with a warp-wide maximum a round: 66 and 25 us; that with full keys, two
-// maxima a round and groups summed through shared memory, as the slow election below has it: 89 and 37 us.)
+// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 42 us forward (28 us
+// without the doubtful tokens, below), on logits alone 15 us, and 12 us backward.  (A warp a token with a warp-wide maximum a
+// round: 66 and 25 us; that with full keys, two maxima a round and groups summed through shared memory: 89 and 37 us.)
 //
 // 24 bits hold every bf16 and fp16 logit, so the choice is exact where neither bias nor groups take part (scores rise with
 // logits).  Otherwise a lane looks at the gap between its and the last lane's value, at the one behind the last elected and at
 // the border between groups.  Where a gap is not wider than what the keys and fp32 lose (and the two do not come from the
-// same logit and bias, where the lower index is right), the whole warp elects for that token again, in
-// fp64: about one token in 450 of random ones.
+// same logit and bias, where the lower index is right), the whole warp elects for that token again, in fp64: about one token
+// in 450 of random ones.
 #pragma once
 #include <math_constants.h>
 
@@ -495,17 +495,17 @@ struct RouterBwdArgs {
 template <typename T, int VPL>
 __global__ void __launch_bounds__(kRouterThreads) router_topk_bwd_kernel(const __grid_constant__ RouterBwdArgs a) {
   const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x * (kRouterThreads / 32) + (threadIdx.x >> 5);
+  const long long t = (long long)blockIdx.x * (kRouterThreads / 32) + (threadIdx.x >> 5);
   if (t >= a.tokens) return;
   const T* row = static_cast<const T*>(a.logits) + t * a.stride;
-  T* out = static_cast<T*>(a.dlogits) + (long long)t * a.experts;
+  T* out = static_cast<T*>(a.dlogits) + t * a.experts;
   int e = -1;
   float lj = -CUDART_INF_F, d = 0.f;
   if (lane < a.top_k) {
-    const long long index = a.indices[(long long)t * a.top_k + lane];
+    const long long index = a.indices[t * a.top_k + lane];
     e = index >= 0 && index < a.experts ? (int)index : -1;
     if (e >= 0) lj = Elem<T>::load1(row + e);
-    d = Elem<T>::load1(static_cast<const T*>(a.dweights) + (long long)t * a.top_k + lane) * a.scale;
+    d = Elem<T>::load1(static_cast<const T*>(a.dweights) + t * a.top_k + lane) * a.scale;
   }
   float g[VPL], chosen;   // the gradients of a run of experts of this lane's; of lane j's chosen expert
 #pragma unroll
