@@ -67,7 +67,8 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
  *   scratch                         device fp64, b200train_clip_scratch_doubles(...) of them
  *   norm                            out, device fp32: n = sqrt(sum of g^2 over all tensors).  Squares are fp32, sums beyond a
  *                                   few hundred of them fp64: an element above 1.8e19 makes n infinite.
- * c = min(1, max_norm / (n + 1e-6)), max_norm >= 0; a NaN norm makes c NaN, an infinite one 0.  No value is read by the host.
+ * c = min(1, max_norm / (n + 1e-6)), max_norm >= 0; a NaN norm makes c NaN, an infinite one 0; max_norm = inf is no limit, c = 1.
+ * No value is read by the host.
  */
 int64_t b200train_clip_scratch_doubles(int64_t tensors, int32_t device);
 

@@ -31,7 +31,8 @@ The steps either side of attention
 ``tests/golden/moe_*.npz`` (made by ``tests/golden/make_golden_moe.py`` from the unmodified module);
 ``rope_fp32`` restates the rotary embedding (``modeling_gpt_oss.py:226-242``) and is pinned against
 the installed function itself in ``tests/test_rope_oracle.py``.  Both are imported by name
-(``oracle.moe_fp32``, ``oracle.rope_fp32``), by the tests and the smoke check only.
+(``oracle.moe_fp32``, ``oracle.rope_fp32``), by the tests and the smoke check only.  ``step_fp64`` restates the
+norm, the router, the gradient clip and their gradients in 64 bits (``tests/test_step_oracle.py``).
 """
 from .eager_fp32 import (  # noqa: F401
     AttnCase,

@@ -207,7 +207,7 @@ clip_apply_kernel(const __grid_constant__ ClipTable t, const double* partials, i
   for (int i = threadIdx.x; i < parts; i += kClipThreads) sum += partials[i];
   const float n = (float)sqrt(block_sum(sum));
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm != nullptr) *norm = n;
-  float scale = max_norm / (n + 1e-6f);
+  float scale = isinf(max_norm) ? 1.f : max_norm / (n + 1e-6f);   // (no limit: nothing is scaled, whatever the norm)
   if (scale >= 1.f) {   // (not where it is NaN: that goes into the gradients)
     if (!kUpdate) return;
     scale = 1.f;

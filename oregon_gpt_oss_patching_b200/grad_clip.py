@@ -8,7 +8,7 @@ synchronises with the host, and both calls can be captured into a graph:
     n = sqrt(sum of g^2),   c = min(1, max_norm / (n + 1e-6)),   g <- c g     or     p <- p - lr c g
 
 ``clip_grad_norm`` stands in for ``torch.nn.utils.clip_grad_norm_`` (2-norm; the same ``c``, the same handling of a norm that
-is not finite); ``clipped_sgd_step`` for a clip followed by ``p -= lr * g``, with two thirds of the memory traffic and one
+is not finite, except that an infinite ``max_norm`` is no limit and never scales); ``clipped_sgd_step`` for a clip followed by ``p -= lr * g``, with two thirds of the memory traffic and one
 rounding instead of two; the gradients stay as they were.  Tensors are bf16, fp16 or fp32, mixed at will, a parameter and
 its gradient of one type, all on one device.  Results are bit-reproducible: every sum has an order fixed by the sizes.
 """
@@ -30,7 +30,7 @@ def _listed(tensors: _Tensors) -> list:
 
 
 def global_grad_norm(tensors: _Tensors) -> torch.Tensor:
-    """The 2-norm of all the tensors' elements together, an fp32 scalar on their device."""
+    """The 2-norm of all the tensors' elements together, an fp32 scalar on their device (0 on the CPU for no tensors)."""
     return _binding.load().global_grad_norm(_listed(tensors))
 
 

@@ -41,20 +41,26 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.
     return _binding.load().rms_norm(x, weight, eps)
 
 
+def _weight_for(norm, x):
+    """The module's weight in a type that goes with ``x``: the module multiplies in fp32 whatever the two types are."""
+    weight = norm.weight
+    return weight if weight.dtype == x.dtype or weight.dtype == torch.float32 else weight.float()
+
+
 def b200_rms_norm_forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
     """Same signature and result as ``GptOssRMSNorm.forward`` (modeling_gpt_oss.py:57-63)."""
-    return rms_norm(hidden_states, self.weight, self.variance_epsilon)
+    return rms_norm(hidden_states, _weight_for(self, hidden_states), self.variance_epsilon)
 
 
 def b200_decoder_layer_forward(self, hidden_states, attention_mask=None, position_ids=None, past_key_values=None, use_cache=False,
                                position_embeddings=None, **kwargs):
     """Same signature and result as ``GptOssDecoderLayer.forward`` (modeling_gpt_oss.py:357-386), its first sum and both norms fused."""
     norm = self.input_layernorm
-    hidden_states, residual = add_rms_norm(hidden_states, None, norm.weight, norm.variance_epsilon)
+    hidden_states, residual = add_rms_norm(hidden_states, None, _weight_for(norm, hidden_states), norm.variance_epsilon)
     hidden_states, _ = self.self_attn(hidden_states=hidden_states, attention_mask=attention_mask, position_ids=position_ids,
                                       past_key_values=past_key_values, use_cache=use_cache, position_embeddings=position_embeddings, **kwargs)
     norm = self.post_attention_layernorm
-    hidden_states, residual = add_rms_norm(hidden_states, residual, norm.weight, norm.variance_epsilon)
+    hidden_states, residual = add_rms_norm(hidden_states, residual, _weight_for(norm, hidden_states), norm.variance_epsilon)
     hidden_states, _ = self.mlp(hidden_states)
     return residual + hidden_states
 

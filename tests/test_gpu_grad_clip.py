@@ -157,6 +157,30 @@ def test_norms_that_are_not_finite():
             assert bool((p.grad[~torch.isnan(p.grad)] == 0).all())
 
 
+def test_no_limit_never_scales():
+    params = make(SIZES["layer"])
+    params[0].grad[3, 5] = float("inf")
+    kept = [p.grad.clone() for p in params]
+    assert float(clip_grad_norm(params, float("inf"))) == float("inf")
+    assert all(torch.equal(p.grad, k) for p, k in zip(params, kept))
+    before = [p.detach().clone() for p in params]
+    clipped_sgd_step(params, 0.5)
+    for p, b, k in list(zip(params, before, kept))[1:]:
+        assert bool(torch.isfinite(p).all()) and not torch.equal(p.detach(), b)
+
+
+def test_offsets_past_32_bits():
+    n = 2 ** 31 + 2 ** 20 + 3
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV, dtype=BF16))
+    p.grad = torch.ones(n, device=DEV, dtype=BF16)
+    p.grad[-1], p.grad[5] = 3.0, -2.0
+    norm = clipped_sgd_step([p], 1.0, float("inf"))
+    assert float(norm) == pytest.approx((n - 2 + 13) ** 0.5, rel=34 * U)
+    assert p[-1] == -3 and p[5] == 2 and p[-2] == -1 and p[2 ** 31] == -1 and float(p.detach().sum(dtype=torch.float64)) == -(n - 2) - 3 + 2
+    clip_grad_norm([p], 0.5 * float(norm))
+    assert p.grad[-1] == 1.5 and p.grad[5] == -1 and float(p.grad.sum(dtype=torch.float64)) == (n - 2) * 0.5 + 1.5 - 1
+
+
 def test_zero_and_tiny_gradients():
     params = make(SIZES["layer"], scale=0.0)
     assert float(check_clip(params, 1.0)) == 0.0

@@ -154,6 +154,33 @@ def test_strides_no_tokens_and_refusals():
         router_topk(big.double(), 2)
 
 
+def test_offsets_past_32_bits():
+    T, E = 8_500_000, 256                           # 2.18e9 logits
+    l = torch.empty(T, E, device=DEV, dtype=BF16).normal_(generator=torch.Generator(device=DEV).manual_seed(1)).requires_grad_(True)
+    w, i = router_topk(l, 8)
+    d = torch.ones_like(w)
+    d[:, 0] = -1
+    (dl,) = torch.autograd.grad(w, l, d)
+    for part in (slice(0, 100), slice(T - 100, T), slice(8_388_600, 8_388_700)):
+        rows = l.detach()[part]
+        ref_w, ref_i = step_fp64.router_topk(rows, 8)
+        assert torch.equal(i[part], ref_i)
+        assert bool(((w.detach()[part].double() - ref_w).abs() <= rounding(ref_w, BF16) + 64 * U * ref_w.abs()).all())
+        ref = step_fp64.router_topk_bwd(rows, ref_i, d[part])
+        assert bool(((dl[part].double() - ref).abs() <= rounding(ref, BF16) + 256 * U).all())
+
+
+def test_a_choice_of_which_only_the_indices_are_used():
+    l = make(5, 32, FP32).requires_grad_(True)
+    w, i = router_topk(l, 4)
+    assert w.requires_grad and not i.requires_grad
+    (g,) = torch.autograd.grad(l.gather(1, i).sum(), l)
+    assert float(g.sum()) == 20
+    w, _ = router_topk(l, 4)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(w.sum(), l, create_graph=True)
+
+
 def test_results_repeat_and_survive_another_stream_and_a_captured_graph():
     l = make(3000, 256, BF16)
     bias = torch.randn(256, device=DEV) * 0.05

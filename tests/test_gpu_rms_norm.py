@@ -160,6 +160,56 @@ def test_results_repeat_and_survive_another_stream_and_a_captured_graph():
     assert all(torch.equal(a, b) for a, b in zip(after, third)) and not torch.equal(after[0], first[0])
 
 
+def test_a_module_s_weight_of_another_type():
+    from transformers.models.gpt_oss.modeling_gpt_oss import GptOssRMSNorm
+    from oregon_gpt_oss_patching_b200.rms_norm import b200_rms_norm_forward
+    mod = GptOssRMSNorm(96, eps=1e-5).to(device=DEV, dtype=BF16)
+    x = torch.randn(5, 96, device=DEV)
+    ref, _ = step_fp64.add_rms_norm(x, None, mod.weight.detach(), 1e-5)
+    y = b200_rms_norm_forward(mod, x)
+    within(y.detach(), ref, 64 * U * ref.abs(), FP32)
+    y.sum().backward()
+    assert mod.weight.grad.dtype == BF16
+
+
+def test_what_is_changed_between_the_passes_is_noticed():
+    x, r, w, dy, dh = make(7, 2880, BF16, BF16)
+    for change in (lambda y, h: h.add_(1), lambda y, h: w.add_(1)):
+        leaves = [t.detach().requires_grad_(True) for t in (x, r)] + [w.requires_grad_(True)]
+        y, h = add_rms_norm(*leaves)
+        with torch.no_grad():
+            change(y, h)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, leaves, dy)
+    w.requires_grad_(False)
+    leaves = [t.detach().requires_grad_(True) for t in (x, r, w)]
+    y, h = add_rms_norm(*leaves)
+    once = torch.autograd.grad((y, h), leaves, (dy, dh), retain_graph=True)
+    again = torch.autograd.grad((y, h), leaves, (dy, dh))
+    assert all(torch.equal(a, b) for a, b in zip(once, again))
+    y, h = add_rms_norm(*leaves)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad((y, h), leaves, (dy, dh), create_graph=True)
+
+
+def test_offsets_past_32_bits():
+    rows, cols = 760_000, 2880                      # 2.19e9 elements
+    x = torch.empty(rows, cols, device=DEV, dtype=BF16).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    w = (1 + 0.1 * torch.randn(cols, device=DEV)).to(BF16)
+    leaf = x.requires_grad_(True)
+    y = rms_norm(leaf, w)
+    (dx,) = torch.autograd.grad(y, leaf, x.detach())
+    for part in (slice(0, 3), slice(rows - 3, rows), slice(745_600, 745_700)):
+        rows_of = x.detach()[part]
+        ref, h = step_fp64.add_rms_norm(rows_of, None, w, 1e-5)
+        within(y.detach()[part], ref, 64 * U * ref.abs(), BF16)
+        ref_dx, _ = step_fp64.add_rms_norm_bwd(h, w, rows_of, None, 1e-5)
+        n = h / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-5)
+        g = h * w.double()
+        size = (n / h).abs().nan_to_num() * (g.abs() + n.abs() * (g * n).abs().mean(-1, keepdim=True))
+        within(dx[part], ref_dx, 128 * U * size, BF16)
+
+
 def test_the_patched_layer_gives_the_model_s_results():
     from transformers import GptOssConfig
     from transformers.models.gpt_oss import modeling_gpt_oss
