@@ -55,7 +55,7 @@ def _binding_command(nvcc: str) -> list:
     return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
             "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
             "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], "-o", BINDING_PATH,
-            os.path.join(CSRC, "train_binding.cpp"), "-L" + lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+            os.path.join(CSRC, "train_binding.cpp"), "-L" + lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <memory>
 #include <new>
 #include <utility>
@@ -18,9 +19,14 @@ namespace {
 using namespace b200train;
 using namespace b200attn::host;
 
+// (asked for several times a call: looked up once a device)
 int sm_count(int device) {
-  int n = 0;
+  static std::atomic<int> known[kMaxDevices];
+  const bool cacheable = device >= 0 && device < kMaxDevices;
+  int n = cacheable ? known[device].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) return 148;
+  if (cacheable) known[device].store(n, std::memory_order_relaxed);
   return n;
 }
 

@@ -9,6 +9,7 @@
 // The module calls the library through addresses it is given (set_library), so that there is one loaded copy of it, the one
 // that the Python side found, checked and reports on.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
@@ -76,6 +77,10 @@ int dtype_code(at::ScalarType t) {
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
 bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
 Tensor copy_of(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
+// A contiguous tensor on x's device, without the dispatcher's way there (half the time of at::empty, and most calls make two to five).
+Tensor empty_on(const Tensor& x, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, x.device(), std::nullopt);
+}
 const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
 // ---------------------------------------------------------------- norm
@@ -129,11 +134,11 @@ Normed norm_forward(const Tensor& x, const std::optional<Tensor>& residual, cons
   Normed n;
   const Rows in(x, cols);
   n.weight = weight.is_contiguous() && aligned16(weight) ? weight : copy_of(weight);
-  n.y = at::empty(x.sizes(), x.options());
+  n.y = empty_on(x, x.sizes(), x.scalar_type());
   Rows r;
   if (residual.has_value()) {
     r = Rows(*residual, cols);
-    n.h = at::empty(x.sizes(), x.options());
+    n.h = empty_on(x, x.sizes(), x.scalar_type());
     n.kept.t = n.h;
     n.kept.stride = cols;
   } else {
@@ -171,12 +176,12 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     const int64_t cols = w.size(0), rows = dy.numel() / cols;
     const int device = dy.get_device(), dtype = dtype_code(dy.scalar_type());
     const Rows dyr(dy, cols), dhr = dh.defined() ? Rows(dh, cols) : Rows();
-    Tensor dx = at::empty(dy.sizes(), dy.options()), dw, scratch;
+    Tensor dx = empty_on(dy, dy.sizes(), dy.scalar_type()), dw, scratch;
     int64_t floats = 0;
     if (ctx->needs_input_grad(residual ? 2 : 1)) {   // (an input that is not there has no place)
-      dw = at::empty(w.sizes(), w.options());
+      dw = empty_on(w, w.sizes(), w.scalar_type());
       floats = lib.norm_scratch_floats(rows, static_cast<int32_t>(cols), dtype, device);
-      scratch = at::empty({floats}, dy.options().dtype(at::kFloat));
+      scratch = empty_on(dy, {floats}, at::kFloat);
     }
     check(lib.add_rms_norm_bwd(data(dyr.t), dyr.stride, data(dhr.t), dhr.stride, data(h), ctx->saved_data["stride"].toInt(), data(w),
                                dx.mutable_data_ptr(), dw.defined() ? dw.mutable_data_ptr() : nullptr,
@@ -221,8 +226,8 @@ std::pair<Tensor, Tensor> router_forward(const Tensor& logits, const std::option
   const int64_t tokens = logits.size(0), experts = logits.size(1);
   Tensor b;
   if (bias.has_value()) b = bias->detach().to(at::kFloat).contiguous();
-  Tensor weights = at::empty({tokens, how.top_k}, logits.options());
-  Tensor indices = at::empty({tokens, how.top_k}, logits.options().dtype(at::kLong));
+  Tensor weights = empty_on(logits, {tokens, how.top_k}, logits.scalar_type());
+  Tensor indices = empty_on(logits, {tokens, how.top_k}, at::kLong);
   check(lib.router_topk(data(logits), logits.stride(0), b.defined() ? b.const_data_ptr<float>() : nullptr, weights.mutable_data_ptr(),
                         indices.mutable_data_ptr<int64_t>(), static_cast<int32_t>(tokens), static_cast<int32_t>(experts),
                         static_cast<int32_t>(how.top_k), static_cast<int32_t>(how.num_groups), static_cast<int32_t>(how.top_groups), how.sigmoid,
@@ -254,7 +259,7 @@ struct RouterTopk : torch::autograd::Function<RouterTopk> {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &indices = saved[1], dweights = grads[0].contiguous();
     const int device = logits.get_device();
-    out[0] = at::empty(logits.sizes(), logits.options());
+    out[0] = empty_on(logits, logits.sizes(), logits.scalar_type());
     check(lib.router_topk_bwd(data(logits), logits.stride(0), indices.const_data_ptr<int64_t>(), data(dweights), out[0].mutable_data_ptr(),
                               static_cast<int32_t>(logits.size(0)), static_cast<int32_t>(logits.size(1)), static_cast<int32_t>(indices.size(1)),
                               ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renormalize"].toBool(),
@@ -324,8 +329,8 @@ struct Output {
   int64_t doubles;
   Output(const Tensor& like, size_t tensors, int device) {
     doubles = lib.clip_scratch_doubles(static_cast<int64_t>(tensors), device);
-    scratch = at::empty({doubles}, like.options().dtype(at::kDouble));
-    norm = at::empty({}, like.options().dtype(at::kFloat));
+    scratch = empty_on(like, {doubles}, at::kDouble);
+    norm = empty_on(like, {}, at::kFloat);
   }
 };
 
