@@ -37,7 +37,8 @@ enum { B200TRAIN_EOVERLAP = -10 }; /* two tensors of one call, one of which is w
  *   weight        (cols), element type `weight_dtype`: `dtype` or B200TRAIN_FP32
  *   y, h          (rows x cols) contiguous, fully overwritten; neither may overlap an input
  * Base pointers 16-byte aligned.  Where cols is a multiple of 16 bytes' worth of elements, the strides must be too;
- * otherwise the inputs must be contiguous (stride == cols).  rows >= 0, 1 <= cols <= B200TRAIN_NORM_MAX_COLS.
+ * otherwise the inputs must be contiguous (stride == cols).  rows >= 0, eps >= 0, 1 <= cols <= B200TRAIN_NORM_MAX_COLS, and
+ * 8 elements less (4 of fp32) where cols is no multiple of 16 bytes' worth.
  */
 int b200train_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                            const void* weight, void* y, void* h, int64_t rows, int32_t cols, float eps, int32_t dtype,

@@ -46,7 +46,8 @@ int launch_dependent(void (*kernel)(P...), unsigned grid, dim3 block, size_t sme
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess ? B200ATTN_OK : B200ATTN_ECUDA;
+  const bool launched = cudaLaunchKernelEx(&config, kernel, args...) == cudaSuccess;
+  return launch_status() == B200ATTN_OK && launched ? B200ATTN_OK : B200ATTN_ECUDA;   // (the error is taken off the thread, as after <<<>>>)
 }
 
 // ---------------------------------------------------------------- norm
@@ -114,8 +115,8 @@ int check_norm_matrix(const void* p, int64_t stride, int64_t rows, int cols, int
   return B200ATTN_OK;
 }
 
-int check_norm(int64_t rows, int cols, int dtype, int weight_dtype, const void* weight) {
-  if (rows < 0 || cols <= 0 || weight == nullptr || !known_dtype(dtype)) return B200ATTN_EINVAL;
+int check_norm(int64_t rows, int cols, int dtype, int weight_dtype, const void* weight, float eps) {
+  if (rows < 0 || cols <= 0 || weight == nullptr || !known_dtype(dtype) || !(eps >= 0.f)) return B200ATTN_EINVAL;
   if (weight_dtype != dtype && weight_dtype != B200TRAIN_FP32) return B200ATTN_EINVAL;
   if (cols > B200TRAIN_NORM_MAX_COLS || rows > (1ll << 40) / cols) return B200ATTN_ESHAPE;
   return aligned16(weight) ? B200ATTN_OK : B200ATTN_EALIGN;
@@ -255,7 +256,7 @@ extern "C" {
 int b200train_add_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                            const void* weight, void* y, void* h, int64_t rows, int32_t cols, float eps, int32_t dtype,
                            int32_t weight_dtype, int32_t device, void* stream) {
-  int rc = check_norm(rows, cols, dtype, weight_dtype, weight);
+  int rc = check_norm(rows, cols, dtype, weight_dtype, weight, eps);
   if (rc) return rc;
   if (rows > 0 && (residual == nullptr) != (h == nullptr)) return B200ATTN_EINVAL;
   if ((rc = check_norm_matrix(x, x_stride, rows, cols, dtype)) || (rc = check_norm_matrix(y, cols, rows, cols, dtype))) return rc;
@@ -292,7 +293,7 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
                                int64_t h_stride, const void* weight, void* dx, void* dweight, float* scratch,
                                int64_t scratch_floats, int64_t rows, int32_t cols, float eps, int32_t dtype,
                                int32_t weight_dtype, int32_t device, void* stream) {
-  int rc = check_norm(rows, cols, dtype, weight_dtype, weight);
+  int rc = check_norm(rows, cols, dtype, weight_dtype, weight, eps);
   if (rc) return rc;
   if ((rc = check_norm_matrix(dy, dy_stride, rows, cols, dtype)) || (rc = check_norm_matrix(h, h_stride, rows, cols, dtype)) ||
       (rc = check_norm_matrix(dx, cols, rows, cols, dtype)))

@@ -9,9 +9,9 @@
 //
 // Both are bound by HBM: clipping cannot do without reading the gradients twice (unless they fit in L2) and writing them once;
 // the folded update reads gradients twice and parameters once and writes the parameters, where clipping first and updating
-// then moves half as much again.  One decoder layer's 823 M bf16 gradients: norm 234 us (7.0 TB/s), clip 780 us (6.3 TB/s, the second read
-// included), update 985 us (6.7 TB/s).
-// (Loads one word at a time between the stores, which the compiler must keep in order: update 1212 us.)
+// then moves half as much again.  One decoder layer's 823 M bf16 gradients: norm 232 us (7.1 TB/s), clip 780 us (6.3 TB/s, the
+// second read included), update 985 us (6.7 TB/s).  (Loads one word at a time between the stores, which the compiler must keep
+// in order: update 1212 us.)
 //
 // The tensors' addresses and sizes travel as a kernel parameter (no copy to the device, nothing to keep alive, nothing for a
 // captured graph to find changed).  Work is cut into chunks of kChunkWords 16-byte words of the 16-byte grid that covers a

@@ -140,7 +140,7 @@ struct RowLane {
   }
 };
 
-// Sums over a row lane.  Warps leave their sums in `part`, whose entries behind the last warp hold zeros; turns alternate, so
+// Sums over a row lane.  Warps leave their sums in `v`, whose entries behind the last warp hold zeros; turns alternate, so
 // that a buffer is written again only when every thread has come past a barrier after reading it.
 struct LaneSums {
   float v[2][kNormBarriers][kNormMaxWarps];

@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kRouterThreads, 4) router_topk_kernel(const __
     if (place == i) won = list[i];
   const bool chosen = there && place < a.top_k;
   int expert = 255 - (int)(won & 255u);
-  float x = chosen ? Elem<T>::load1(row + expert) : -CUDART_INF_F;
+  float x = chosen && won != 0u ? Elem<T>::load1(row + expert) : -CUDART_INF_F;
   if (!kExact) {
     float b = 0.f, v = x;
     if (kValues && chosen) {

@@ -34,11 +34,11 @@ def test_norm_arguments_are_validated(lib):
     buf = torch.zeros(1 << 12, dtype=torch.float32)
     p = buf.data_ptr()
 
-    def fwd(x=p, xs=64, r=None, rs=0, w=p, y=p, h=None, rows=2, cols=64, dtype=0, wdtype=0):
-        return lib.b200train_add_rms_norm(x, xs, r, rs, w, y, h, rows, cols, 1e-5, dtype, wdtype, 0, None)
+    def fwd(x=p, xs=64, r=None, rs=0, w=p, y=p, h=None, rows=2, cols=64, dtype=0, wdtype=0, eps=1e-5):
+        return lib.b200train_add_rms_norm(x, xs, r, rs, w, y, h, rows, cols, eps, dtype, wdtype, 0, None)
 
     assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(y=None) == -1
-    assert fwd(rows=-1) == -1 and fwd(cols=0) == -1
+    assert fwd(rows=-1) == -1 and fwd(cols=0) == -1 and fwd(eps=-1.0) == -1 and fwd(eps=float("nan")) == -1
     assert fwd(dtype=3) == -1 and fwd(dtype=-1) == -1 and fwd(dtype=0, wdtype=1) == -1 and fwd(dtype=2, wdtype=0) == -1
     assert fwd(r=p, rs=64) == -1 and fwd(h=p) == -1                       # a residual and its sum come together
     assert fwd(cols=16385, xs=16385) == -2
