@@ -2,9 +2,9 @@
 // include/b200train.h and the router of include/b200moe.h.  Host code alone, one extension module.
 //
 // The attention and expert wrappers do this in Python; these operators are called once or twice a layer on little data (or on
-// hundreds of small tensors), where the host's time is what a caller waits for: a norm of a few rows takes 9 us of it here and 14 us
-// through Python and ctypes, a forward with its backward 62 us and 94 us (45 us of them autograd's own), the routing of a few
-// tokens 7 us and 22 us, clipping 48 gradients 20 us and 50 us.
+// hundreds of small tensors), where the host's time is what a caller waits for: a norm of a few rows takes 7.5 us of it here and 14 us
+// through Python and ctypes, a forward with its backward 60 us and 94 us (45 us of them autograd's own), the routing of a few
+// tokens 6 us and 22 us, clipping 48 gradients 18 us and 50 us.
 //
 // The module calls the library through addresses it is given (set_library), so that there is one loaded copy of it, the one
 // that the Python side found, checked and reports on.

@@ -67,6 +67,78 @@ def test_gradients_of_the_fused_step_are_the_model_s():
         assert float((fused[name] - ref).norm() / ref.norm()) <= 1.5 * off + 2.0 ** -7, (name, off)
 
 
+def test_nothing_is_kept_after_a_step():
+    """Forward alone, forward and backward, clip and update: when their tensors are dropped, the device's memory is as it was."""
+    import gc
+    from oregon_gpt_oss_patching_b200.grad_clip import clip_grad_norm, clipped_sgd_step
+    from oregon_gpt_oss_patching_b200.moe_router import router_topk
+    from oregon_gpt_oss_patching_b200.rms_norm import add_rms_norm, rms_norm
+    x, r = (torch.randn(2000, 2880, device="cuda").bfloat16().requires_grad_(True) for _ in range(2))
+    w = torch.nn.Parameter(torch.ones(2880, device="cuda", dtype=torch.bfloat16))
+    logits = torch.randn(2000, 32, device="cuda", requires_grad=True)
+
+    def step(backward):
+        y, h = add_rms_norm(x, r, w)
+        z, same = add_rms_norm(y, None, w)
+        t, _ = router_topk(logits, 4)
+        if backward:
+            (rms_norm(z, w).sum() + (h + same).sum() + t.sum()).backward()
+            clip_grad_norm([w, x, r, logits], 1.0)
+            clipped_sgd_step([w], 0.0, 1.0)
+            for p in (w, x, r, logits):
+                p.grad = None
+
+    step(True)
+    gc.collect()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    gc.disable()           # (cycles would have to wait for the collector)
+    try:
+        for backward in (False, True, False, True):
+            step(backward)
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() == before
+    finally:
+        gc.enable()
+
+
+def test_threads_and_streams_at_once():
+    """Four threads, each on a stream of its own, run all operators on their own tensors: the same results as one after the other."""
+    import threading
+    from oregon_gpt_oss_patching_b200.grad_clip import clipped_sgd_step
+    from oregon_gpt_oss_patching_b200.moe_router import router_topk
+    from oregon_gpt_oss_patching_b200.rms_norm import add_rms_norm
+
+    def work(seed, out):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            x, r, dy, dh = (torch.randn(500, 2880, device="cuda", generator=g).bfloat16() for _ in range(4))
+            w = torch.nn.Parameter(torch.ones(2880, device="cuda", dtype=torch.bfloat16))
+            logits = torch.randn(500, 64, device="cuda", generator=g)
+            for _ in range(10):
+                x.requires_grad_(True)
+                y, h = add_rms_norm(x, r, w)
+                gx, w.grad = torch.autograd.grad((y, h), (x, w), (dy, dh))
+                norm = clipped_sgd_step([w], 0.1, 1.0)
+                t, i = router_topk(logits, 6, scoring="sigmoid", bias=logits[0], num_groups=4, top_groups=2)
+                x = (x + gx).detach()
+            out[seed] = [v.detach().cpu() for v in (x, w, norm, t, i)]
+            stream.synchronize()
+
+    one, many = {}, {}
+    for seed in range(4):
+        work(seed, one)
+    threads = [threading.Thread(target=work, args=(seed, many)) for seed in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert one.keys() == many.keys()
+    for seed in one:
+        assert all(torch.equal(a, b) for a, b in zip(one[seed], many[seed]))
+
+
 def test_a_clipped_update_is_a_clip_and_an_update():
     from oregon_gpt_oss_patching_b200.grad_clip import clipped_sgd_step
     model = _model(layers=1)
