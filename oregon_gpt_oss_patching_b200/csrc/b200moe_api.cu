@@ -93,10 +93,13 @@ void launch_router(RouterArgs a, cudaStream_t st) {
 }
 template <typename T, int VPL>
 void launch_router(RouterBwdArgs a, cudaStream_t st) {
-  a.vector_in = on_grid(a.logits, a.stride, VPL, sizeof(T));
-  a.vector_out = on_grid(a.dlogits, a.experts, VPL, sizeof(T));
-  const int grid = (int)(((long long)a.tokens + kRouterThreads / 32 - 1) / (kRouterThreads / 32));
-  router_topk_bwd_kernel<T, VPL><<<grid, kRouterThreads, 0, st>>>(a);
+  constexpr int RL = VPL == 1 ? 4 : 8, RUNS = VPL <= 2 ? 1 : VPL / 2;
+  const bool quick = a.top_k <= kQuickLanes;
+  a.vector_in = on_grid(a.logits, a.stride, quick ? RL : VPL, sizeof(T));
+  a.vector_out = on_grid(a.dlogits, a.experts, quick ? RL : VPL, sizeof(T));
+  const int tokens = quick ? kQuickTokens : kRouterThreads / 32, grid = (int)(((long long)a.tokens + tokens - 1) / tokens);
+  if (quick) router_topk_bwd_kernel<T, RL, RUNS, kQuickLanes><<<grid, kRouterThreads, 0, st>>>(a);
+  else router_topk_bwd_kernel<T, VPL, 1, 32><<<grid, kRouterThreads, 0, st>>>(a);
 }
 // by how many experts a lane holds
 template <typename T, typename Args>

@@ -12,9 +12,9 @@
 // experts (whole lanes to a group) into keys: the upper 24 bits of the value in an order of unsigned integers, and 255 - expert
 // below, so that keys differ and the larger one is the one to elect.  It sorts them by eights with a network, keeps the best 8
 // (or 4, where top_k allows), and three exchanges between the lanes leave the token's best in all of them.  Instructions bound
-// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 42 us forward (28 us
-// without the doubtful tokens, below), on logits alone 15 us, and 12 us backward.  (A warp a token with a warp-wide maximum a
-// round: 66 and 25 us; that with full keys, two maxima a round and groups summed through shared memory: 89 and 37 us.)
+// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 39 us forward (28 us
+// without the doubtful tokens, below), on logits alone 15 us, and 8 us backward.  (A warp a token with a warp-wide maximum a
+// round: 66, 25 and 12 us; that with full keys, two maxima a round and groups summed through shared memory: 89 and 37 us.)
 //
 // 24 bits hold every bf16 and fp16 logit, so the choice is exact where neither bias nor groups take part (scores rise with
 // logits).  Otherwise a lane looks at the gap between its and the last lane's value, at the one behind the last elected and at
@@ -78,86 +78,89 @@ struct RouterArgs {
   float scale;
 };
 
+// The value of a key.
+__device__ __forceinline__ double value_of(unsigned long long key) {
+  return __longlong_as_double((long long)((key >> 63) ? key & ~(1ull << 63) : ~key));
+}
+
 // The slow election: any groups and top_k, values in fp64, a whole warp a token; lane j's return is the j-th expert.  `row` (shared,
-// of this warp) holds the values by expert, later their keys.  Loops instead of registers keep the code small: it is cold when a
-// doubtful token of the quick election comes to it, and instruction fetches are what it waits for (the same unrolled over
-// registers, with an fp32 try first, took the kernel 48 us instead of 42).
+// of this warp) holds the values' keys by expert, 0 where an expert cannot be elected any more.  One token waits for it, so
+// latency counts: no branch keeps neighbouring experts' exponentials apart, groups are looked through by integer compares, and a
+// lane knows its best until that is elected.  (12700 cycles a token of 256 experts in 8 groups; with doubles in shared memory, a
+// division by the group's size and every lane's list walked in every round 17200.)
 template <typename T>
 __device__ __noinline__ int elect_slowly(const RouterArgs& a, const T* logits, int lane, unsigned long long* row) {
-  const bool by_logit = a.bias == nullptr && a.groups == 1;   // scores rise with logits
-  double m = 0.0, z = 1.0;
-  if (!a.sigmoid && !by_logit) {
-    float top = -CUDART_INF_F;
-    for (int e = lane; e < a.experts; e += 32) {
-      const float l = Elem<T>::load1(logits + e);
-      top = l > top || l != l ? l : top;
-    }
-    m = lanes_max(top, 32);
-  }
-  // the first turn sums the softmax, the second writes the values
-  for (int turn = a.sigmoid || by_logit ? 1 : 0; turn < 2; ++turn) {
-    double sum = 0.0;
-#pragma unroll 1
-    for (int e = lane; e < a.experts; e += 32) {
-      const float l = Elem<T>::load1(logits + e);
-      double v = l;
-      if (!by_logit && l != -CUDART_INF_F) {
-        const double x = exp(a.sigmoid ? -v : v - m);
-        sum += x;
-        v = (a.sigmoid ? 1.0 : x) / (a.sigmoid ? 1.0 + x : z) + (a.bias != nullptr ? (double)a.bias[e] : 0.0);
+  if (a.bias == nullptr && a.groups == 1) {   // scores rise with logits
+    for (int e = lane; e < a.experts; e += 32) row[e] = (unsigned long long)order_key(Elem<T>::load1(logits + e)) << 32;
+  } else {
+    double m = 0.0, part_of = 1.0;   // the softmax's maximum, and one over its sum
+    if (!a.sigmoid) {
+      float top = -CUDART_INF_F;
+      for (int e = lane; e < a.experts; e += 32) {
+        const float l = Elem<T>::load1(logits + e);
+        top = l > top || l != l ? l : top;
       }
-      row[e] = (unsigned long long)__double_as_longlong(v);
+      m = lanes_max(top, 32);
+      double sum = 0.0;
+#pragma unroll 4
+      for (int e = lane; e < a.experts; e += 32) {
+        const float l = Elem<T>::load1(logits + e);
+        sum += l == -CUDART_INF_F ? 0.0 : exp((double)l - m);
+      }
+      sum = lanes_add(sum, 32);
+      part_of = sum == 0.0 ? 0.0 : 1.0 / sum;
     }
-    if (turn == 0) z = lanes_add(sum, 32);
+#pragma unroll 4
+    for (int e = lane; e < a.experts; e += 32) {
+      const float l = Elem<T>::load1(logits + e);
+      const double x = exp(a.sigmoid ? -(double)l : (double)l - m);
+      const double v = (a.sigmoid ? __drcp_rn(1.0 + x) : x * part_of) + (a.bias != nullptr ? (double)a.bias[e] : 0.0);
+      row[e] = order_key(l == -CUDART_INF_F ? -CUDART_INF : v);
+    }
   }
-  __syncwarp();
-  uint32_t open = 0xffffffffu;
-  const int size = a.experts / a.groups;
   if (a.groups > 1) {
+    __syncwarp();
     int part = 32;   // lanes that look through one group
     while (part * a.groups > 32) part >>= 1;
-    double best = -CUDART_INF, next = -CUDART_INF;
-    bool number = true;
-    if (lane / part < a.groups) {
+    const int size = a.experts / a.groups, mine = lane / part;
+    unsigned long long best = 0ull, next = 0ull;
+    if (mine < a.groups) {
       for (int i = lane % part; i < size; i += part) {
-        const double v = __longlong_as_double((long long)row[lane / part * size + i]);
-        number = number && v == v;
-        next = fmax(next, fmin(best, v));
-        best = fmax(best, v);
+        const unsigned long long k = row[mine * size + i];
+        next = max(next, min(best, k));
+        best = max(best, k);
       }
     }
     for (int o = part >> 1; o > 0; o >>= 1) {
-      const double f = __shfl_xor_sync(0xffffffffu, best, o), n = __shfl_xor_sync(0xffffffffu, next, o);
-      next = fmax(fmin(best, f), fmax(next, n));
-      best = fmax(best, f);
-      number = __shfl_xor_sync(0xffffffffu, (int)number, o) && number;
+      const unsigned long long f = __shfl_xor_sync(0xffffffffu, best, o), n = __shfl_xor_sync(0xffffffffu, next, o);
+      next = max(min(best, f), max(next, n));
+      best = max(best, f);
     }
-    double sum = !number ? CUDART_NAN : next == -CUDART_INF ? best : best + next;
-    sum = __shfl_sync(0xffffffffu, sum, lane * part & 31);   // lane g ranks group g
-    const unsigned long long key = order_key(sum);
+    // (the key of -inf: no second expert that is not masked; there is none at all in a group of one)
+    const double sum = next <= order_key(-CUDART_INF) ? value_of(best) : value_of(best) + value_of(next);
+    const unsigned long long key = order_key(__shfl_sync(0xffffffffu, sum, lane * part & 31));   // lane g ranks group g
     int ahead = 0;
     for (int g = 0; g < a.groups; ++g) {
       const unsigned long long other = __shfl_sync(0xffffffffu, key, g);
       ahead += other > key || (other == key && g < lane);
     }
-    open = __ballot_sync(0xffffffffu, lane < a.groups && ahead < a.top_groups);
+    const uint32_t open = __ballot_sync(0xffffffffu, lane < a.groups && ahead < a.top_groups);
     __syncwarp();
+    if (mine < a.groups && !(open >> mine & 1u))
+      for (int i = lane % part; i < size; i += part) row[mine * size + i] = 0ull;
   }
-  // keys: 0 for an expert of a closed group and for one elected already
-#pragma unroll 1
-  for (int e = lane; e < a.experts; e += 32)
-    row[e] = a.groups == 1 || (open >> (e / size) & 1u) ? order_key(__longlong_as_double((long long)row[e])) : 0ull;
-  int elected = 0;
-#pragma unroll 1
+  __syncwarp();
+  unsigned long long best = 0ull;
+  int at = a.experts, elected = 0;
+  bool stale = true;
   for (int j = 0; j < a.top_k; ++j) {
-    unsigned long long best = 0ull;
-    int at = a.experts;
-#pragma unroll 2
-    for (int e = lane; e < a.experts; e += 32) {   // (the lane's own entries: no other lane writes them)
-      const unsigned long long k = row[e];
-      if (k > best) {
-        best = k;
-        at = e;
+    if (stale) {   // (the lane's best was elected: look for the next one among its own, which no other lane writes)
+      best = 0ull;
+#pragma unroll 4
+      for (int e = lane; e < a.experts; e += 32) {
+        const unsigned long long k = row[e];
+        at = k > best ? e : at;
+        best = max(best, k);
       }
     }
     // the largest upper half, of those the largest lower half, of those the lowest expert
@@ -165,7 +168,8 @@ __device__ __noinline__ int elect_slowly(const RouterArgs& a, const T* logits, i
     const bool ahead = upper == __reduce_max_sync(0xffffffffu, upper);
     const uint32_t top = __reduce_max_sync(0xffffffffu, ahead ? lower : 0u);
     const int winner = (int)__reduce_min_sync(0xffffffffu, ahead && lower == top ? (uint32_t)at : 0xffffffffu);
-    if (lane == (winner & 31)) row[winner] = 0ull;
+    stale = at == winner;
+    if (stale) row[winner] = 0ull;
     if (lane == j) elected = winner;
   }
   __syncwarp();
@@ -492,61 +496,79 @@ struct RouterBwdArgs {
 // With d_j = scale * dw_j and, renormalised, r_j = s_j / sum_S s and d_j <- (d_j - sum_S d r) / sum_S s:
 //   sigmoid   dl_j = d_j s_j (1 - s_j) for the chosen, 0 elsewhere
 //   softmax   dl_i = s_i (d_i - sum_S d s), d_i = 0 where i is not chosen; renormalised that is r_j (d_j - sum_S d r), 0 elsewhere
-template <typename T, int VPL>
+//
+// W lanes serve a token (8, or 32 where top_k is above 8): lane j has the j-th chosen expert, and all of them write the row, RUNS
+// runs of RL experts a lane.
+template <typename T, int RL, int RUNS, int W>
 __global__ void __launch_bounds__(kRouterThreads) router_topk_bwd_kernel(const __grid_constant__ RouterBwdArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long t = (long long)blockIdx.x * (kRouterThreads / 32) + (threadIdx.x >> 5);
-  if (t >= a.tokens) return;
-  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
-  T* out = static_cast<T*>(a.dlogits) + t * a.experts;
+  const int lane = threadIdx.x & 31, place = lane % W;
+  const long long warp_token = ((long long)blockIdx.x * (kRouterThreads / 32) + (threadIdx.x >> 5)) * (32 / W);
+  if (warp_token >= a.tokens) return;   // (whole warps leave)
+  const long long t = warp_token + lane / W;
+  const bool there = t < a.tokens;
+  const T* row = static_cast<const T*>(a.logits) + (there ? t : warp_token) * a.stride;
   int e = -1;
   float lj = -CUDART_INF_F, d = 0.f;
-  if (lane < a.top_k) {
-    const long long index = a.indices[t * a.top_k + lane];
+  if (there && place < a.top_k) {
+    const long long index = a.indices[t * a.top_k + place];
     e = index >= 0 && index < a.experts ? (int)index : -1;
     if (e >= 0) lj = Elem<T>::load1(row + e);
-    d = Elem<T>::load1(static_cast<const T*>(a.dweights) + t * a.top_k + lane) * a.scale;
+    d = Elem<T>::load1(static_cast<const T*>(a.dweights) + t * a.top_k + place) * a.scale;
   }
-  float g[VPL], chosen;   // the gradients of a run of experts of this lane's; of lane j's chosen expert
+  float g[RUNS][RL], chosen;   // the gradients of this lane's runs; of its chosen expert
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) g[i] = 0.f;
-  const int first = lane * VPL, n = max(0, min(VPL, a.experts - first));
+  for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+    for (int i = 0; i < RL; ++i) g[r][i] = 0.f;
   if (a.sigmoid) {
     const float x = expf(-fabsf(lj)), s = (lj >= 0.f ? 1.f : x) / (1.f + x);   // (no overflow on either side)
     const float slope = x / ((1.f + x) * (1.f + x));
     if (a.renormalize) {
-      const float sum = lanes_add(e >= 0 ? s : 0.f, 32);
-      const float dot = lanes_add(e >= 0 ? d * s : 0.f, 32);
+      const float sum = lanes_add(e >= 0 ? s : 0.f, W);
+      const float dot = lanes_add(e >= 0 ? d * s : 0.f, W);
       d = sum == 0.f ? 0.f : (d - dot / sum) / sum;
     }
     chosen = d * slope;
   } else if (a.renormalize) {
-    const float m = lanes_max(lj, 32);
+    const float m = lanes_max(lj, W);
     const float s = lj == -CUDART_INF_F ? 0.f : expf(lj - m);
-    const float sum = lanes_add(s, 32);
+    const float sum = lanes_add(s, W);
     const float r = sum == 0.f ? 0.f : s / sum;
-    chosen = r * (d - lanes_add(e >= 0 ? d * r : 0.f, 32));
+    chosen = r * (d - lanes_add(e >= 0 ? d * r : 0.f, W));
   } else {
-    float l[VPL], z = 0.f;
-    load_run<T, VPL>(row + first, n, a.vector_in != 0 && n == VPL, l);
-    float m = l[0];
+    float m = -CUDART_INF_F, z = 0.f;
 #pragma unroll
-    for (int i = 1; i < VPL; ++i) m = l[i] > m || l[i] != l[i] ? l[i] : m;
-    m = lanes_max(m, 32);
+    for (int r = 0; r < RUNS; ++r) {
+      const int first = (r * W + place) * RL, n = a.experts - first;
+      load_run<T, RL>(row + first, n, a.vector_in != 0 && n >= RL, g[r]);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      g[i] = l[i] == -CUDART_INF_F ? 0.f : expf(l[i] - m);
-      z += g[i];
+      for (int i = 0; i < RL; ++i) m = g[r][i] > m || g[r][i] != g[r][i] ? g[r][i] : m;
     }
-    z = lanes_add(z, 32);
-    const float s = lj == -CUDART_INF_F || z == 0.f ? 0.f : expf(lj - m) / z;
-    const float dot = lanes_add(e >= 0 ? d * s : 0.f, 32);
-    chosen = s * (d - dot);
+    m = lanes_max(m, W);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) g[i] = z == 0.f ? 0.f : -(g[i] / z) * dot;
+    for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+      for (int i = 0; i < RL; ++i) {
+        g[r][i] = g[r][i] == -CUDART_INF_F ? 0.f : expf(g[r][i] - m);
+        z += g[r][i];
+      }
+    z = lanes_add(z, W);
+    const float s = lj == -CUDART_INF_F || z == 0.f ? 0.f : expf(lj - m) / z;
+    const float dot = lanes_add(e >= 0 ? d * s : 0.f, W);
+    chosen = s * (d - dot);
+    const float back = z == 0.f ? 0.f : -dot / z;
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+      for (int i = 0; i < RL; ++i) g[r][i] *= back;
   }
   // the whole row first, then the chosen experts over it (stores of one warp in this order)
-  store_run<T, VPL>(out + first, n, a.vector_out != 0 && n == VPL, g);
+  T* out = static_cast<T*>(a.dlogits) + t * a.experts;
+#pragma unroll
+  for (int r = 0; r < RUNS; ++r) {
+    const int first = (r * W + place) * RL, n = there ? a.experts - first : 0;
+    store_run<T, RL>(out + first, n, a.vector_out != 0 && n >= RL, g[r]);
+  }
   __syncwarp();
   if (e >= 0) Elem<T>::store1(out + e, chosen);
 }
