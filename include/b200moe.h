@@ -104,7 +104,8 @@ enum { B200MOE_BF16 = 0, B200MOE_FP16 = 1, B200MOE_FP32 = 2 };
  *   with groups > 1 the experts form that many equal runs, a run's value is the sum of its two largest v that are not
  *   -inf, and only the experts of the top_groups largest runs are eligible
  *   indices[t,:] = the top_k largest v of the eligible, in falling order; ties, here and between runs, go to the lowest
- *   index; NaN ranks above everything.  The order is that of the real numbers (fp64 where fp32 cannot tell two apart).
+ *   index; NaN ranks above everything.  The order is that of the real numbers (that of the logits where
+ *   there is no bias, that of v in fp64 where fp32 cannot tell two apart).
  *   weights[t,j] = scale * s / (renormalize ? sum of the chosen s : 1), of the chosen; 0 where that sum is 0
  *   logits    (tokens x experts) of `dtype`, `stride` elements from row to row;  bias: device fp32 (experts) or NULL
  *   weights   out, (tokens x top_k) of `dtype`;  indices: out, device int64 (tokens x top_k)

@@ -49,6 +49,8 @@ def router_topk(logits, top_k, sigmoid=False, bias=None, groups=1, top_groups=1,
         closed = torch.ones_like(value, dtype=torch.bool).scatter(1, kept, False).repeat_interleave(parts.shape[-1], dim=1)
         # masked experts of an eligible group still rank above every expert of a closed one
         rank = torch.where(closed, 2, masked.int())
+        if bias is None:   # scores rise with logits, past the point where 64 bits tell them apart
+            v = l
         order = v.sort(dim=1, descending=True, stable=True).indices
         order = order.gather(1, rank.gather(1, order).sort(dim=1, stable=True).indices)
         indices = order[:, :top_k]

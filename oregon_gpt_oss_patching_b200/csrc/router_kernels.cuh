@@ -12,12 +12,11 @@
 // experts (whole lanes to a group) into keys: the upper 24 bits of the value in an order of unsigned integers, and 255 - expert
 // below, so that keys differ and the larger one is the one to elect.  It sorts them by eights with a network, keeps the best 8
 // (or 4, where top_k allows), and three exchanges between the lanes leave the token's best in all of them.  Instructions bound
-// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 39 us forward (28 us
-// without the doubtful tokens, below), on logits alone 15 us, and 8 us backward.  (A warp a token with a warp-wide maximum a
+// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 37 us forward (26 us
+// without the doubtful tokens, below), on logits alone 12.5 us, and 8 us backward.  (A warp a token with a warp-wide maximum a
 // round: 66, 25 and 12 us; that with full keys, two maxima a round and groups summed through shared memory: 89 and 37 us.)
 //
-// 24 bits hold every bf16 and fp16 logit, so the choice is exact where neither bias nor groups take part (scores rise with
-// logits).  Otherwise a lane looks at the gap between its and the last lane's value, at the one behind the last elected and at
+// 24 bits hold every bf16 and fp16 logit, so the order is exact where no bias takes part (scores rise with logits).  Otherwise a lane looks at the gap between its and the last lane's value, at the one behind the last elected and at
 // the border between groups.  Where a gap is not wider than what the keys and fp32 lose (and the two do not come from the
 // same logit and bias, where the lower index is right), the whole warp elects for that token again, in fp64: about one token
 // in 450 of random ones.
@@ -39,11 +38,11 @@ constexpr int kRouterMaxGroups = 32;     // one lane a group at least
 constexpr int kQuickLanes = 8;           // of a token
 constexpr int kQuickTokens = kRouterThreads / kQuickLanes;
 
-// fp32 and fp64 values as unsigned keys in the same order; NaN above everything (as torch.topk has it), -0 as 0.
+// fp32 and fp64 values as unsigned keys in the same order; NaN above everything (as torch.topk has it), -0 as 0.  (An fp32 sum makes
+// 0 of -0 and the one positive NaN, 0x7fffffff, of any.)
 __device__ __forceinline__ uint32_t order_key(float v) {
-  const uint32_t b = __float_as_uint(v + 0.f);
-  if (v != v) return 0xffffffffu;
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  const int b = __float_as_int(v + 0.f);
+  return (uint32_t)(b ^ (b >> 31 | (int)0x80000000));
 }
 __device__ __forceinline__ unsigned long long order_key(double v) {
   const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
@@ -146,8 +145,9 @@ __device__ __noinline__ int elect_slowly(const RouterArgs& a, const T* logits, i
     }
     const uint32_t open = __ballot_sync(0xffffffffu, lane < a.groups && ahead < a.top_groups);
     __syncwarp();
-    if (mine < a.groups && !(open >> mine & 1u))
-      for (int i = lane % part; i < size; i += part) row[mine * size + i] = 0ull;
+    if (mine < a.groups && (a.bias == nullptr || !(open >> mine & 1u)))   // (without a bias the order is that of the logits again)
+      for (int e = mine * size + lane % part; e < (mine + 1) * size; e += part)
+        row[e] = open >> mine & 1u ? (unsigned long long)order_key(Elem<T>::load1(logits + e)) << 32 : 0ull;
   }
   __syncwarp();
   unsigned long long best = 0ull;
@@ -311,7 +311,8 @@ __device__ __forceinline__ void write_choice(const RouterArgs& a, long long at, 
   }
 }
 
-// The quick election.  A lane holds RUNS runs of RL experts and a list of LL keys (top_k <= LL).  kValues: a bias or groups take part.
+// The quick election.  A lane holds RUNS runs of RL experts and a list of LL keys (top_k <= LL).  kValues: a bias or groups take part
+// (without a bias the values are there for the groups' sums, and the keys are those of the logits).
 template <typename T, int RL, int RUNS, int LL, bool kValues>
 __global__ void __launch_bounds__(kRouterThreads, 4) router_topk_kernel(const __grid_constant__ RouterArgs a) {
   constexpr bool kExact = !kValues && sizeof(T) == 2;
@@ -347,9 +348,9 @@ __global__ void __launch_bounds__(kRouterThreads, 4) router_topk_kernel(const __
     if (!kValues || x == -CUDART_INF_F) return x;
     return (a.sigmoid ? quick_sigmoid(x) : __fdividef(expf(x - m), z)) + b;
   };
-  const bool grouped = kValues && a.groups > 1;
+  const bool grouped = kValues && a.groups > 1, by_logit = !kValues || a.bias == nullptr;
+  const bool exact = by_logit && sizeof(T) == 2;          // the keys tell any two experts apart
   float best_v = -CUDART_INF_F, next_v = -CUDART_INF_F;   // the two largest values of this lane's part of a group
-  bool numbers = true;                                    // none of them is NaN
   uint32_t list[LL], lost = 0u;
 #pragma unroll
   for (int i = 0; i < LL; ++i) list[i] = 0u;
@@ -365,11 +366,10 @@ __global__ void __launch_bounds__(kRouterThreads, 4) router_topk_kernel(const __
       const int e = first + r * RL + i;
       const bool has = r * RL + i < mine;
       const float v = has ? value(l[r][i], bias[i]) : -CUDART_INF_F;
-      key[i] = has ? make_key(v, e) : 0u;
+      key[i] = has ? make_key(by_logit ? l[r][i] : v, e) : 0u;
       if (grouped) {
         next_v = fmaxf(next_v, fminf(best_v, v));
         best_v = fmaxf(best_v, v);
-        numbers = numbers && v == v;
       }
     }
     sort_keys<RL>(key);
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kRouterThreads, 4) router_topk_kernel(const __
     if (a.top_groups < a.groups) {   // the narrowest of the gaps between an open group and a closed one
       const float in = -lanes_max(open ? -sum : -CUDART_INF_F, kQuickLanes), out = lanes_max(open ? -CUDART_INF_F : sum, kQuickLanes);
       const float most = lanes_max(slack, kQuickLanes);
-      sure = (in - out > most || (in == -CUDART_INF_F && out == -CUDART_INF_F)) && numbers;
+      sure = (in - out > most || (in == -CUDART_INF_F && out == -CUDART_INF_F)) && list[0] < 0xffffff00u;   // (no NaN: the maxima pass it by)
     }
     if (!open) {
 #pragma unroll
@@ -426,15 +426,15 @@ __global__ void __launch_bounds__(kRouterThreads, 4) router_topk_kernel(const __
   float x = chosen && won != 0u ? Elem<T>::load1(row + expert) : -CUDART_INF_F;
   if (!kExact) {
     float b = 0.f, v = x;
-    if (kValues && chosen) {
-      b = a.bias != nullptr ? a.bias[expert] : 0.f;
+    if (!by_logit && chosen) {
+      b = a.bias[expert];
       v = value(x, b);
     }
     const float pv = __shfl_up_sync(0xffffffffu, v, 1, kQuickLanes), px = __shfl_up_sync(0xffffffffu, x, 1, kQuickLanes);
     const float pb = __shfl_up_sync(0xffffffffu, b, 1, kQuickLanes);
-    const float error = kValues ? value_error(a.sigmoid) * (1.f + fabsf(v)) : 0.f;
-    if (place > 0 && chosen) sure = sure && ((x == -CUDART_INF_F && px == -CUDART_INF_F) || (px == x && pb == b) || pv - v > error);
-    if (place == a.top_k - 1) {   // the best of those left out: no one's value is above its key's
+    const float error = by_logit ? 0.f : value_error(a.sigmoid) * (1.f + fabsf(v));
+    if (!exact && place > 0 && chosen) sure = sure && ((x == -CUDART_INF_F && px == -CUDART_INF_F) || (px == x && pb == b) || pv - v > error);
+    if (!exact && place == a.top_k - 1) {   // the best of those left out: no one's value is above its key's
       uint32_t behind = lost;
 #pragma unroll
       for (int i = 1; i < LL; ++i)

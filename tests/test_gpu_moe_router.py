@@ -126,6 +126,15 @@ def test_values_that_are_not_numbers_give_a_valid_choice():
                 assert bool((i.sort(1).values.diff(dim=1) > 0).all())
                 fine = [t for t in range(64) if t not in (3, 4, 5, 6)]
                 assert not bool(torch.isnan(w[fine]).any())
+    for dtype, bits in ((BF16, -64), (FP32, -4194304)):      # a NaN with its sign bit set is one like any other
+        m = make(64, 40, dtype).contiguous()
+        m.view(torch.int16 if dtype == BF16 else torch.int32)[2, 11] = bits
+        assert bool(torch.isnan(m[2, 11]))
+        assert int(router_topk(m, 4)[1][2, 0]) == 11
+        assert int(router_topk(m, 4, scoring="sigmoid", num_groups=4, top_groups=2)[1][2, 0]) == 11
+        # groups go by scores, and a softmax over a NaN has no score that is a number: the first two groups; in them by logits
+        i = router_topk(m, 4, num_groups=4, top_groups=2)[1][2]
+        assert int(i[0]) == 11 and bool((i < 20).all())
     w, i = router_topk(l, 4)
     assert int(i[3, 0]) == 7 and i[4].tolist() == [0, 1, 2, 3] and int(i[5, 0]) == 9
 
