@@ -125,9 +125,19 @@ void check_norm(const char* name, const Tensor& x, const std::optional<Tensor>& 
   TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int32_t>::max(), name, ": rows of ", x.size(-1), " elements");
 }
 
+// A weight as the kernels read it: contiguous, on the 16-byte grid.
+Tensor on_grid(const Tensor& w) { return w.is_contiguous() && aligned16(w) ? w : copy_of(w); }
+
+// A saved value that comes back through a hook (an offload, a compression) may lie otherwise in memory than it did: each is laid
+// out for the kernels again, once it is known to be what was saved.
+void check_saved(const char* name, const Tensor& saved, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+  TORCH_CHECK(saved.sizes() == sizes && saved.scalar_type() == type && saved.device() == device, name, ": a saved tensor came back as ",
+              saved.sizes(), ", ", saved.dtype(), ", ", saved.device(), "; saved were ", sizes, ", ", type, ", ", device);
+}
+
 struct Normed {
   Tensor y, h;      // h undefined without a residual
-  Rows kept;        // what the backward reads as h
+  Tensor kept;      // what the backward reads as h
   Tensor weight;
 };
 
@@ -136,16 +146,15 @@ Normed norm_forward(const Tensor& x, const std::optional<Tensor>& residual, cons
   const int device = x.get_device();
   Normed n;
   const Rows in(x, cols);
-  n.weight = weight.is_contiguous() && aligned16(weight) ? weight : copy_of(weight);
+  n.weight = on_grid(weight);
   n.y = empty_on(x, x.sizes(), x.scalar_type());
   Rows r;
   if (residual.has_value()) {
     r = Rows(*residual, cols);
     n.h = empty_on(x, x.sizes(), x.scalar_type());
-    n.kept.t = n.h;
-    n.kept.stride = cols;
+    n.kept = n.h;
   } else {
-    n.kept = in;
+    n.kept = in.t;
   }
   check(lib.add_rms_norm(data(in.t), in.stride, data(r.t), r.stride, data(n.weight), n.y.mutable_data_ptr(),
                          n.h.defined() ? n.h.mutable_data_ptr() : nullptr, x.numel() / cols, static_cast<int32_t>(cols),
@@ -163,7 +172,8 @@ std::shared_ptr<N> new_node() {
 
 struct AddRmsNormBackward : Node {
   SavedVariable h, weight;
-  int64_t stride = 0;
+  std::vector<int64_t> saved_sizes;   // of h
+  at::ScalarType weight_type = at::kFloat;
   double eps = 0.0;
   std::string name() const override { return "AddRmsNormBackward"; }
   void release_variables() override {
@@ -177,10 +187,13 @@ struct AddRmsNormBackward : Node {
     const Tensor none;
     const bool residual = task_should_compute_output(1);
     if (!dy.defined()) return {dh, residual ? dh : none, none};   // the norm was not used: the stream's gradient passes through
-    const Tensor hs = h.unpack(shared_from_this()), w = weight.unpack();
-    const int64_t cols = w.size(0), rows = dy.numel() / cols;
+    const int64_t cols = dy.size(-1), rows = dy.numel() / cols;
     const int device = dy.get_device(), dtype = dtype_code(dy.scalar_type());
-    const Rows dyr(dy, cols), dhr = dh.defined() ? Rows(dh, cols) : Rows();
+    const Tensor saved = h.unpack(shared_from_this()), saved_weight = weight.unpack();
+    check_saved("add_rms_norm", saved, saved_sizes, dy.scalar_type(), dy.device());
+    check_saved("add_rms_norm", saved_weight, {cols}, weight_type, dy.device());
+    const Tensor w = on_grid(saved_weight);
+    const Rows hs(saved, cols), dyr(dy, cols), dhr = dh.defined() ? Rows(dh, cols) : Rows();
     Tensor dx = empty_on(dy, dy.sizes(), dy.scalar_type()), dw, scratch;
     int64_t floats = 0;
     if (task_should_compute_output(2)) {
@@ -188,7 +201,7 @@ struct AddRmsNormBackward : Node {
       floats = lib.norm_scratch_floats(rows, static_cast<int32_t>(cols), dtype, device);
       scratch = empty_on(dy, {floats}, at::kFloat);
     }
-    check(lib.add_rms_norm_bwd(data(dyr.t), dyr.stride, data(dhr.t), dhr.stride, data(hs), stride, data(w), dx.mutable_data_ptr(),
+    check(lib.add_rms_norm_bwd(data(dyr.t), dyr.stride, data(dhr.t), dhr.stride, data(hs.t), hs.stride, data(w), dx.mutable_data_ptr(),
                                dw.defined() ? dw.mutable_data_ptr() : nullptr, scratch.defined() ? scratch.mutable_data_ptr<float>() : nullptr,
                                floats, rows, static_cast<int32_t>(cols), static_cast<float>(eps), dtype, dtype_code(w.scalar_type()), device,
                                stream_of(device)),
@@ -208,11 +221,12 @@ std::pair<Tensor, Tensor> differentiable_norm(const Tensor& x, const std::option
   }
   auto node = new_node<AddRmsNormBackward>();
   node->set_next_edges(torch::autograd::collect_next_edges(x, residual.has_value() ? *residual : Tensor(), weight));
-  node->stride = n.kept.stride;
+  node->saved_sizes = n.kept.sizes().vec();
+  node->weight_type = n.weight.scalar_type();
   node->eps = eps;
   torch::autograd::set_history(n.y, node);
   if (h.defined()) torch::autograd::set_history(h, node);
-  node->h = residual.has_value() ? SavedVariable(h, true) : SavedVariable(n.kept.t, false);
+  node->h = residual.has_value() ? SavedVariable(h, true) : SavedVariable(n.kept, false);
   node->weight = SavedVariable(n.weight, false);
   return {n.y, h};
 }
@@ -262,6 +276,7 @@ Tensor row_major(const Tensor& logits) { return logits.stride(1) == 1 || logits.
 
 struct RouterTopkBackward : Node {
   SavedVariable logits, indices;
+  int64_t experts = 0;
   bool sigmoid = false, renormalize = false;
   double scale = 1.0;
   std::string name() const override { return "RouterTopkBackward"; }
@@ -273,7 +288,10 @@ struct RouterTopkBackward : Node {
   variable_list apply(variable_list&& grads) override {
     TORCH_CHECK(!at::GradMode::is_enabled(), "router_topk cannot be differentiated twice");
     if (!grads[0].defined()) return {Tensor()};
-    const Tensor l = logits.unpack(), chosen = indices.unpack(), dweights = grads[0].contiguous();
+    const Tensor dweights = grads[0].contiguous(), saved = logits.unpack(), saved_indices = indices.unpack();
+    check_saved("router_topk", saved, {dweights.size(0), experts}, dweights.scalar_type(), dweights.device());
+    check_saved("router_topk", saved_indices, dweights.sizes(), at::kLong, dweights.device());
+    const Tensor l = row_major(saved), chosen = saved_indices.contiguous();
     const int device = l.get_device();
     Tensor dlogits = empty_on(l, l.sizes(), l.scalar_type());
     check(lib.router_topk_bwd(data(l), l.stride(0), chosen.const_data_ptr<int64_t>(), data(dweights), dlogits.mutable_data_ptr(),
@@ -310,6 +328,7 @@ std::pair<Tensor, Tensor> router_topk(const Tensor& logits, int64_t top_k, const
   if (differentiable) {
     auto node = new_node<RouterTopkBackward>();
     node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->experts = experts;
     node->sigmoid = how.sigmoid;
     node->renormalize = renormalize;
     node->scale = scale;
