@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <limits>
 #include <optional>
 #include <string>
@@ -341,6 +342,98 @@ std::pair<Tensor, Tensor> router_topk(const Tensor& logits, int64_t top_k, const
 
 // ---------------------------------------------------------------- clip
 
+// The bytes that a strided tensor takes: `size` of them at every sum of multiples of the dimensions' strides.
+struct Span {
+  struct Dim {
+    int64_t stride, n;
+  };
+  int64_t begin = 0, bytes = 0, size = 0;   // from the first byte to behind the last one; of an element
+  std::vector<Dim> dims;                    // of more than one index, the largest stride first
+  explicit Span(const Tensor& t) {
+    size = static_cast<int64_t>(t.element_size());
+    if (t.numel() == 0) return;
+    begin = reinterpret_cast<int64_t>(t.const_data_ptr());
+    bytes = size;
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.size(d) > 1 && t.stride(d) > 0) {   // (a stride of 0 adds no byte)
+        dims.push_back({t.stride(d) * size, t.size(d)});
+        bytes += dims.back().stride * (dims.back().n - 1);
+      }
+    std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+  }
+};
+
+// Whether no byte of `a` is one of `b`, which lies `shift` behind it: the indices of the largest stride S differ by k, and for each k
+// that brings the rest of the two near each other, that rest is compared, k * S further on.  Where strides nest, as in
+// slices and permutations of one buffer, that is a few steps; where `steps` run out the answer is no.
+bool apart(const Span::Dim* a, const Span::Dim* a_end, int64_t a_bytes, const Span::Dim* b, const Span::Dim* b_end, int64_t b_bytes, int64_t shift,
+           int& steps) {
+  if (shift >= a_bytes || shift + b_bytes <= 0) return true;
+  if ((a == a_end && b == b_end) || --steps < 0) return false;
+  const int64_t s = std::max(a != a_end ? a->stride : 0, b != b_end ? b->stride : 0);
+  int64_t least = 0, most = 0;   // k: b's index less a's
+  if (a != a_end && a->stride == s) {
+    least = -(a->n - 1);
+    a_bytes -= (a++->n - 1) * s;
+  }
+  if (b != b_end && b->stride == s) {
+    most = b->n - 1;
+    b_bytes -= (b++->n - 1) * s;
+  }
+  const auto down = [s](int64_t v) { return v >= 0 ? v / s : -((-v + s - 1) / s); };
+  least = std::max(least, down(-b_bytes - shift) + 1);
+  most = std::min(most, down(a_bytes - 1 - shift));
+  for (int64_t k = least; k <= most; ++k)
+    if (!apart(a, a_end, a_bytes, b, b_end, b_bytes, shift + k * s, steps)) return false;
+  return true;
+}
+constexpr int kApartSteps = 1 << 14;
+
+bool share_memory(const Span& a, const Span& b) {
+  int steps = kApartSteps;
+  return a.bytes != 0 && b.bytes != 0 &&
+         !apart(a.dims.data(), a.dims.data() + a.dims.size(), a.bytes, b.dims.data(), b.dims.data() + b.dims.size(), b.bytes, b.begin - a.begin, steps);
+}
+// Whether two elements of a tensor share memory (but for strides of 0).
+bool shares_with_itself(const Span& t) {
+  int64_t rest = t.bytes;
+  const Span::Dim* end = t.dims.data() + t.dims.size();
+  for (const Span::Dim* d = t.dims.data(); d != end; ++d) {
+    rest -= (d->n - 1) * d->stride;
+    for (int64_t k = 1; k < d->n && k * d->stride < rest; ++k) {
+      int steps = kApartSteps;
+      if (!apart(d + 1, end, rest, d + 1, end, rest, k * d->stride, steps)) return true;
+    }
+  }
+  return false;
+}
+
+// Refuses tensors to be written that have memory twice, share it with one another or with one that is read.  Contiguous tensors are
+// looked through by the library; where there are others it sees copies of them.
+void check_apart(const char* name, const std::vector<Tensor>& written, const std::vector<Tensor>& read) {
+  bool packed = false;
+  for (const Tensor& t : written) {
+    if (t.is_contiguous()) continue;
+    packed = true;
+    for (int64_t d = 0; d < t.dim(); ++d)
+      TORCH_CHECK_VALUE(t.stride(d) != 0 || t.size(d) <= 1, name, ": a tensor with a stride of 0 cannot be written in place");
+    TORCH_CHECK_VALUE(!shares_with_itself(Span(t)), name, ": a tensor whose elements share memory cannot be written in place");
+  }
+  for (const Tensor& t : read) packed = packed || !t.is_contiguous();
+  if (!packed) return;
+  std::vector<std::pair<Span, bool>> all;
+  all.reserve(written.size() + read.size());
+  for (const Tensor& t : written) all.emplace_back(Span(t), true);
+  for (const Tensor& t : read) all.emplace_back(Span(t), false);
+  std::sort(all.begin(), all.end(), [](const auto& a, const auto& b) { return a.first.begin < b.first.begin; });
+  for (size_t i = 0; i < all.size(); ++i)
+    for (size_t j = i + 1; j < all.size() && all[j].first.begin < all[i].first.begin + all[i].first.bytes; ++j)
+      if (all[i].second || all[j].second) {
+        const int rc = share_memory(all[i].first, all[j].first) ? B200TRAIN_EOVERLAP : 0;
+        check(rc, name);
+      }
+}
+
 // The arrays that the library reads: addresses, counts and types of contiguous tensors on one device.
 struct Table {
   std::vector<int64_t> grads, params, counts;
@@ -406,14 +499,12 @@ Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm) {
   for (const Tensor& p : parameters) {
     const Tensor& g = p.grad();
     if (!g.defined()) continue;
-    for (int64_t d = 0; d < g.dim(); ++d)
-      TORCH_CHECK_VALUE(g.layout() != at::kStrided || g.stride(d) != 0 || g.size(d) <= 1,
-                        "clip_grad_norm: a gradient with a stride of 0 cannot be scaled in place");
     grads.push_back(g);
     packed.push_back(g.layout() == at::kStrided ? dense(g) : g);
   }
   if (grads.empty()) return at::zeros({}, at::kFloat);
   const Table t("clip_grad_norm", packed, nullptr);
+  check_apart("clip_grad_norm", grads, {});
   Output out(packed[0], packed.size(), t.device);
   check(lib.clip_grads(t.grads.data(), t.counts.data(), t.dtypes.data(), static_cast<int64_t>(packed.size()), limit,
                        out.scratch.mutable_data_ptr<double>(), out.doubles, out.norm.mutable_data_ptr<float>(), t.device, stream_of(t.device)),
@@ -428,18 +519,20 @@ Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm) {
 Tensor clipped_sgd_step(const std::vector<Tensor>& parameters, double lr, double max_norm) {
   at::NoGradGuard no_grad;
   const float limit = limit_of("clipped_sgd_step", max_norm);
-  std::vector<Tensor> params, grads, packed;
+  std::vector<Tensor> params, packed, grads, packed_grads;
   for (const Tensor& p : parameters) {
     const Tensor& g = p.grad();
     if (!g.defined()) continue;
     TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "clipped_sgd_step: a gradient must have its parameter's type, got ", g.dtype(), " for ",
                      p.dtype());
     params.push_back(p);
-    grads.push_back(g.layout() == at::kStrided ? dense(g) : g);
+    grads.push_back(g);
+    packed_grads.push_back(g.layout() == at::kStrided ? dense(g) : g);
     packed.push_back(dense(p));
   }
   if (params.empty()) return at::zeros({}, at::kFloat);
-  const Table t("clipped_sgd_step", grads, &packed);
+  const Table t("clipped_sgd_step", packed_grads, &packed);
+  check_apart("clipped_sgd_step", params, grads);
   Output out(grads[0], grads.size(), t.device);
   check(lib.clipped_sgd(t.grads.data(), t.params.data(), t.counts.data(), t.dtypes.data(), static_cast<int64_t>(grads.size()),
                         static_cast<float>(lr), limit, out.scratch.mutable_data_ptr<double>(), out.doubles, out.norm.mutable_data_ptr<float>(),
@@ -462,4 +555,6 @@ PYBIND11_MODULE(_train_binding, m) {
   m.def("global_grad_norm", &global_grad_norm);
   m.def("clip_grad_norm", &clip_grad_norm);
   m.def("clipped_sgd_step", &clipped_sgd_step);
+  m.def("share_memory", [](const Tensor& a, const Tensor& b) { return share_memory(Span(a), Span(b)); });
+  m.def("shares_with_itself", [](const Tensor& t) { return shares_with_itself(Span(t)); });
 }

@@ -37,7 +37,8 @@ def global_grad_norm(tensors: _Tensors) -> torch.Tensor:
 def clip_grad_norm(parameters: _Tensors, max_norm: float) -> torch.Tensor:
     """Scale the parameters' gradients in place so that their global 2-norm is at most ``max_norm``; returns the norm before.
 
-    Parameters without a gradient are passed over.  Gradients that share memory are refused (one parameter given twice).
+    Parameters without a gradient are passed over.  Gradients that share an element (one parameter given twice, overlapping views), or
+    one that has an element twice, are refused before anything is written; views that only lie in between each other are fine.
     """
     return _binding.load().clip_grad_norm(_listed(parameters), max_norm)
 
@@ -45,6 +46,7 @@ def clip_grad_norm(parameters: _Tensors, max_norm: float) -> torch.Tensor:
 def clipped_sgd_step(parameters: _Tensors, lr: float, max_norm: float = float("inf")) -> torch.Tensor:
     """``p -= lr * c * p.grad`` for every parameter that has a gradient, c from the global norm of the gradients; returns the norm.
 
-    The gradients are not changed.  Parameters and gradients that share memory are refused.
+    The gradients are not changed.  A parameter that shares an element with another one or with a gradient, or has one twice, is
+    refused before anything is written, and so are contiguous gradients that share memory.
     """
     return _binding.load().clipped_sgd_step(_listed(parameters), lr, max_norm)
