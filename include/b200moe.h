@@ -106,7 +106,8 @@ enum { B200MOE_BF16 = 0, B200MOE_FP16 = 1, B200MOE_FP32 = 2 };
  *   indices[t,:] = the top_k largest v of the eligible, in falling order; ties, here and between runs, go to the lowest
  *   index; NaN ranks above everything.  The order is that of the real numbers (that of the logits where
  *   there is no bias, that of v in fp64 where fp32 cannot tell two apart).
- *   weights[t,j] = scale * s / (renormalize ? sum of the chosen s : 1), of the chosen; 0 where that sum is 0
+ *   weights[t,j] = scale * s / (renormalize ? sum of the chosen s : 1), of the chosen; 0 where all of them are masked.  Shares are right
+ *   however low the logits lie: equal ones at the type's lowest value have equal shares
  *   logits    (tokens x experts) of `dtype`, `stride` elements from row to row;  bias: device fp32 (experts) or NULL
  *   weights   out, (tokens x top_k) of `dtype`;  indices: out, device int64 (tokens x top_k)
  * 1 <= top_k <= min(32, top_groups * experts / groups), experts <= 256, groups <= 32 divides experts.

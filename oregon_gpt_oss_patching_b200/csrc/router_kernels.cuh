@@ -289,13 +289,19 @@ __device__ __forceinline__ void merge_keys(uint32_t (&a)[LL], const uint32_t (&b
   }
 }
 
+// Sigmoid scores as numbers: s = e^min(x,0) / (1 + e^-|x|) over e^shift.  Shares s_j / sum_S s do not depend on the shift, and with the
+// largest chosen logit m in it, where that is negative, they are right however low the logits lie (e^-89 is no fp32 number).
+__device__ __forceinline__ float share_shift(float m) { return m < 0.f && m != -CUDART_INF_F ? m : 0.f; }
+__device__ __forceinline__ float sigmoid_over(float x, float shift) { return expf(fminf(x, 0.f) - shift) / (1.f + expf(-fabsf(x))); }
+
 // The weights of the elected: lane j (of `width` that serve the token) has the j-th expert and its logit x, `chosen` for
 // j < top_k.  m and z: the maximum and the sum of the softmax over all experts (not needed where it is renormalised).
 template <typename T>
 __device__ __forceinline__ void write_choice(const RouterArgs& a, long long at, bool chosen, int width, int expert, float x, float m, float z) {
   float s;
   if (a.sigmoid) {
-    s = chosen ? 1.f / (1.f + expf(-x)) : 0.f;
+    const float shift = a.renormalize ? share_shift(lanes_max(chosen ? x : -CUDART_INF_F, width)) : 0.f;
+    s = chosen ? sigmoid_over(x, shift) : 0.f;
   } else {
     if (a.renormalize) m = lanes_max(chosen ? x : -CUDART_INF_F, width);
     s = chosen && x != -CUDART_INF_F ? expf(x - m) : 0.f;
@@ -493,8 +499,8 @@ struct RouterBwdArgs {
   float scale;
 };
 
-// With d_j = scale * dw_j and, renormalised, r_j = s_j / sum_S s and d_j <- (d_j - sum_S d r) / sum_S s:
-//   sigmoid   dl_j = d_j s_j (1 - s_j) for the chosen, 0 elsewhere
+// With d_j = scale * dw_j and r_j = s_j / sum_S s:
+//   sigmoid   dl_j = d_j s_j (1 - s_j) for the chosen, 0 elsewhere; renormalised that is r_j (d_j - sum_S d r) (1 - s_j)
 //   softmax   dl_i = s_i (d_i - sum_S d s), d_i = 0 where i is not chosen; renormalised that is r_j (d_j - sum_S d r), 0 elsewhere
 //
 // W lanes serve a token (8, or 32 where top_k is above 8): lane j has the j-th chosen expert, and all of them write the row, RUNS
@@ -521,14 +527,15 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_bwd_kernel(const _
 #pragma unroll
     for (int i = 0; i < RL; ++i) g[r][i] = 0.f;
   if (a.sigmoid) {
-    const float x = expf(-fabsf(lj)), s = (lj >= 0.f ? 1.f : x) / (1.f + x);   // (no overflow on either side)
-    const float slope = x / ((1.f + x) * (1.f + x));
+    const float x = expf(-fabsf(lj)), rest = (lj >= 0.f ? x : 1.f) / (1.f + x);   // 1 - s (no overflow on either side)
     if (a.renormalize) {
-      const float sum = lanes_add(e >= 0 ? s : 0.f, W);
-      const float dot = lanes_add(e >= 0 ? d * s : 0.f, W);
-      d = sum == 0.f ? 0.f : (d - dot / sum) / sum;
+      const float s = sigmoid_over(lj, share_shift(lanes_max(lj, W)));   // (0 where there is no expert)
+      const float sum = lanes_add(s, W);
+      const float r = sum == 0.f ? 0.f : s / sum;
+      chosen = r * (d - lanes_add(e >= 0 ? d * r : 0.f, W)) * rest;
+    } else {
+      chosen = d * sigmoid_over(lj, 0.f) * rest;
     }
-    chosen = d * slope;
   } else if (a.renormalize) {
     const float m = lanes_max(lj, W);
     const float s = lj == -CUDART_INF_F ? 0.f : expf(lj - m);
