@@ -104,7 +104,7 @@ enum { B200MOE_BF16 = 0, B200MOE_FP16 = 1, B200MOE_FP32 = 2 };
  *   with groups > 1 the experts form that many equal runs, a run's value is the sum of its two largest v that are not
  *   -inf, and only the experts of the top_groups largest runs are eligible
  *   indices[t,:] = the top_k largest v of the eligible, in falling order; ties, here and between runs, go to the lowest
- *   index; NaN ranks above everything.  The order is that of the real numbers (that of the logits where
+ *   index; NaN ranks above everything (a softmax over a logit of +inf makes every v but those of masked experts NaN).  The order is that of the real numbers (that of the logits where
  *   there is no bias, that of v in fp64 where fp32 cannot tell two apart).
  *   weights[t,j] = scale * s / (renormalize ? sum of the chosen s : 1), of the chosen; 0 where all of them are masked.  Shares are right
  *   however low the logits lie: equal ones at the type's lowest value have equal shares

@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(kRouterThreads, 4) router_topk_kernel(const __
     if (a.top_groups < a.groups) {   // the narrowest of the gaps between an open group and a closed one
       const float in = -lanes_max(open ? -sum : -CUDART_INF_F, kQuickLanes), out = lanes_max(open ? -CUDART_INF_F : sum, kQuickLanes);
       const float most = lanes_max(slack, kQuickLanes);
-      sure = (in - out > most || (in == -CUDART_INF_F && out == -CUDART_INF_F)) && list[0] < 0xffffff00u;   // (no NaN: the maxima pass it by)
+      // (no NaN, in a logit or a bias or from a softmax over +inf: the maxima pass it by)
+      sure = (in - out > most || (in == -CUDART_INF_F && out == -CUDART_INF_F)) && list[0] < 0xffffff00u && z == z;
     }
     if (!open) {
 #pragma unroll

@@ -1,4 +1,4 @@
-"""The router far out: sigmoid scores of large negative logits.
+"""The router far out: sigmoid scores of large negative logits, infinite logits in front of groups.
 
 Tolerances.  u = 2^-24.  A weight is a quotient of exponentials whose arguments differ by at most the row's spread D: their
 rounding gives D u, the exponentials, sums and quotients 64 u more (as in the router's other tests).  Below the smallest normal
@@ -13,6 +13,7 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 U = 2.0 ** -24
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+INF = float("inf")
 
 
 def rounding(ref, dtype):
@@ -67,3 +68,24 @@ def test_masks_of_the_type_s_lowest_value(dtype, scoring):
     assert dl[0, :5].tolist() == [-0.5, -0.25, 0.0, 0.75, 0.0]                     # (d - 3) / 4
     slope = 0.5 * (1.0 if scoring == "softmax" else 1 / (1 + 2.718281828459045))    # r (d - 1.5), times 1 - s
     assert dl[1, 7].item() == pytest.approx(-0.5 * slope, rel=2.0 ** -7) and dl[1, 20].item() == pytest.approx(0.5 * slope, rel=2.0 ** -7)
+
+
+@pytest.mark.parametrize("groups,top_groups", [(8, 3), (4, 2), (2, 1), (16, 5)])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_an_infinite_logit_does_not_open_a_masked_group(groups, top_groups, with_bias, dtype):
+    """A softmax over +inf has no score that is a number: every expert that is not masked ranks alike, and groups follow their
+    lowest index; a group that is masked as a whole comes last, in every form of the election."""
+    l = (torch.randn(20, 64, generator=torch.Generator().manual_seed(5)) * 2).to(device=DEV, dtype=dtype)
+    size = 64 // groups
+    l[:, :size] = -INF                                   # the first group is masked
+    l[::2, 2 * size - 1] = INF
+    l[1::4, 63] = INF
+    bias = torch.linspace(-1, 1, 64, device=DEV) if with_bias else None
+    k = min(4, size)
+    _, i = router_topk(l, k, bias=bias, num_groups=groups, top_groups=top_groups)
+    # (on the CPU: what torch's sort does with NaN on a GPU depends on the sort's size)
+    _, ref = step_fp64.router_topk(l.cpu(), k, bias=None if bias is None else bias.cpu(), groups=groups, top_groups=top_groups)
+    assert torch.equal(i.cpu(), ref)
+    if top_groups < groups:
+        assert bool((i >= size).all())
