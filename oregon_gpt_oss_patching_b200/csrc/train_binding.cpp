@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -68,6 +69,16 @@ void set_library(const std::unordered_map<std::string, uintptr_t>& a) {
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed: ", lib.strerror(rc), " (code ", rc, ")"); }
 
+// Forward-mode derivatives would be lost here without a word: nothing below looks at a tangent.
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool has_tangent(const std::optional<Tensor>& t) { return t.has_value() && has_tangent(*t); }
+template <typename... T>
+void check_no_tangent(const char* name, const T&... tensors) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(tensors) || ...), name, " has no forward-mode derivative");
+}
+// Whether any tensor can have a tangent: asked once where there are many of them.
+bool tangents_exist() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+
 // B200TRAIN_* and B200MOE_* (the same numbers), -1 for any other type
 int dtype_code(at::ScalarType t) {
   switch (t) {
@@ -124,6 +135,7 @@ void check_norm(const char* name, const Tensor& x, const std::optional<Tensor>& 
                       residual->dtype(), ", ", residual->device());
   TORCH_CHECK_VALUE(eps >= 0.0, name, ": eps must not be negative, got ", eps);
   TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int32_t>::max(), name, ": rows of ", x.size(-1), " elements");
+  check_no_tangent(name, x, residual, weight);
 }
 
 // A weight as the kernels read it: contiguous, on the 16-byte grid.
@@ -321,6 +333,7 @@ std::pair<Tensor, Tensor> router_topk(const Tensor& logits, int64_t top_k, const
   if (bias.has_value())
     TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == experts && bias->device() == logits.device() && bias->is_floating_point(),
                       "router_topk: bias must be ", experts, " floating point values on ", logits.device());
+  check_no_tangent("router_topk", logits, bias);
   const Routing how{top_k, num_groups, top_groups, scoring == "sigmoid", renormalize, scale};
   const bool differentiable = at::GradMode::is_enabled() && logits.requires_grad();
   at::NoGradGuard no_grad;   // the choice has no gradient: nothing that leads to it is recorded
@@ -411,16 +424,12 @@ bool shares_with_itself(const Span& t) {
 // Refuses tensors to be written that have memory twice, share it with one another or with one that is read.  Contiguous tensors are
 // looked through by the library; where there are others it sees copies of them.
 void check_apart(const char* name, const std::vector<Tensor>& written, const std::vector<Tensor>& read) {
-  bool packed = false;
   for (const Tensor& t : written) {
     if (t.is_contiguous()) continue;
-    packed = true;
     for (int64_t d = 0; d < t.dim(); ++d)
       TORCH_CHECK_VALUE(t.stride(d) != 0 || t.size(d) <= 1, name, ": a tensor with a stride of 0 cannot be written in place");
     TORCH_CHECK_VALUE(!shares_with_itself(Span(t)), name, ": a tensor whose elements share memory cannot be written in place");
   }
-  for (const Tensor& t : read) packed = packed || !t.is_contiguous();
-  if (!packed) return;
   std::vector<std::pair<Span, bool>> all;
   all.reserve(written.size() + read.size());
   for (const Tensor& t : written) all.emplace_back(Span(t), true);
@@ -481,7 +490,11 @@ Tensor global_grad_norm(const std::vector<Tensor>& tensors) {
   if (tensors.empty()) return at::zeros({}, at::kFloat);
   std::vector<Tensor> packed;
   packed.reserve(tensors.size());
-  for (const Tensor& t : tensors) packed.push_back(dense(t));
+  const bool tangents = tangents_exist();
+  for (const Tensor& t : tensors) {
+    if (tangents) check_no_tangent("global_grad_norm", t);
+    packed.push_back(dense(t));
+  }
   const Table t("global_grad_norm", packed, nullptr);
   Output out(packed[0], packed.size(), t.device);
   check(lib.grad_norm(t.grads.data(), t.counts.data(), t.dtypes.data(), static_cast<int64_t>(packed.size()), out.scratch.mutable_data_ptr<double>(),
@@ -494,17 +507,21 @@ Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm) {
   at::NoGradGuard no_grad;
   const float limit = limit_of("clip_grad_norm", max_norm);
   std::vector<Tensor> grads, packed;
+  const bool tangents = tangents_exist();
+  bool copied = false;
   grads.reserve(parameters.size());
   packed.reserve(parameters.size());
   for (const Tensor& p : parameters) {
     const Tensor& g = p.grad();
     if (!g.defined()) continue;
+    if (tangents) check_no_tangent("clip_grad_norm", g);
     grads.push_back(g);
     packed.push_back(g.layout() == at::kStrided ? dense(g) : g);
+    copied = copied || !packed.back().is_same(g);
   }
   if (grads.empty()) return at::zeros({}, at::kFloat);
   const Table t("clip_grad_norm", packed, nullptr);
-  check_apart("clip_grad_norm", grads, {});
+  if (copied) check_apart("clip_grad_norm", grads, {});
   Output out(packed[0], packed.size(), t.device);
   check(lib.clip_grads(t.grads.data(), t.counts.data(), t.dtypes.data(), static_cast<int64_t>(packed.size()), limit,
                        out.scratch.mutable_data_ptr<double>(), out.doubles, out.norm.mutable_data_ptr<float>(), t.device, stream_of(t.device)),
@@ -519,20 +536,27 @@ Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm) {
 Tensor clipped_sgd_step(const std::vector<Tensor>& parameters, double lr, double max_norm) {
   at::NoGradGuard no_grad;
   const float limit = limit_of("clipped_sgd_step", max_norm);
-  std::vector<Tensor> params, packed, grads, packed_grads;
+  std::vector<Tensor> params, grads, packed;
+  const bool tangents = tangents_exist();
+  bool copied = false;
   for (const Tensor& p : parameters) {
     const Tensor& g = p.grad();
     if (!g.defined()) continue;
+    if (tangents) check_no_tangent("clipped_sgd_step", p, g);
     TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "clipped_sgd_step: a gradient must have its parameter's type, got ", g.dtype(), " for ",
                      p.dtype());
     params.push_back(p);
-    grads.push_back(g);
-    packed_grads.push_back(g.layout() == at::kStrided ? dense(g) : g);
+    grads.push_back(g.layout() == at::kStrided ? dense(g) : g);
     packed.push_back(dense(p));
+    copied = copied || !grads.back().is_same(g) || !packed.back().is_same(p);
   }
   if (params.empty()) return at::zeros({}, at::kFloat);
-  const Table t("clipped_sgd_step", packed_grads, &packed);
-  check_apart("clipped_sgd_step", params, grads);
+  const Table t("clipped_sgd_step", grads, &packed);
+  if (copied) {
+    std::vector<Tensor> read;
+    for (const Tensor& p : params) read.push_back(p.grad());
+    check_apart("clipped_sgd_step", params, read);
+  }
   Output out(grads[0], grads.size(), t.device);
   check(lib.clipped_sgd(t.grads.data(), t.params.data(), t.counts.data(), t.dtypes.data(), static_cast<int64_t>(grads.size()),
                         static_cast<float>(lr), limit, out.scratch.mutable_data_ptr<double>(), out.doubles, out.norm.mutable_data_ptr<float>(),
