@@ -52,15 +52,34 @@ def b200_rms_norm_forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
     return rms_norm(hidden_states, _weight_for(self, hidden_states), self.variance_epsilon)
 
 
+def _plain_call(norm) -> bool:
+    """Whether calling the module would do no more than ``b200_rms_norm_forward``: no hook, wrapper or other module would be passed by."""
+    hooks = torch.nn.modules.module
+    return (getattr(type(norm), "forward", None) is b200_rms_norm_forward and type(norm).__call__ is torch.nn.Module.__call__
+            and "forward" not in norm.__dict__ and norm._compiled_call_impl is None
+            and not (norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks
+                     or hooks._global_forward_hooks or hooks._global_forward_pre_hooks or hooks._global_backward_hooks
+                     or hooks._global_backward_pre_hooks))
+
+
+def _add_norm(norm, x, residual):
+    """``(norm(h), h)`` with h = x + residual: one fused call, or a sum and a call of the module where that does more than its forward."""
+    if _plain_call(norm):
+        return add_rms_norm(x, residual, _weight_for(norm, x), norm.variance_epsilon)
+    h = x if residual is None else residual + x
+    return norm(h), h
+
+
 def b200_decoder_layer_forward(self, hidden_states, attention_mask=None, position_ids=None, past_key_values=None, use_cache=False,
                                position_embeddings=None, **kwargs):
-    """Same signature and result as ``GptOssDecoderLayer.forward`` (modeling_gpt_oss.py:357-386), its first sum and both norms fused."""
-    norm = self.input_layernorm
-    hidden_states, residual = add_rms_norm(hidden_states, None, _weight_for(norm, hidden_states), norm.variance_epsilon)
+    """Same signature and result as ``GptOssDecoderLayer.forward`` (modeling_gpt_oss.py:357-386), its first sum and both norms fused.
+
+    A norm with hooks (which may gather its weight first), a forward of its own or another module in its place is called as a module.
+    """
+    hidden_states, residual = _add_norm(self.input_layernorm, hidden_states, None)
     hidden_states, _ = self.self_attn(hidden_states=hidden_states, attention_mask=attention_mask, position_ids=position_ids,
                                       past_key_values=past_key_values, use_cache=use_cache, position_embeddings=position_embeddings, **kwargs)
-    norm = self.post_attention_layernorm
-    hidden_states, residual = add_rms_norm(hidden_states, residual, _weight_for(norm, hidden_states), norm.variance_epsilon)
+    hidden_states, residual = _add_norm(self.post_attention_layernorm, hidden_states, residual)
     hidden_states, _ = self.mlp(hidden_states)
     return residual + hidden_states
 
