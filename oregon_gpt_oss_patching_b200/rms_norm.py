@@ -63,8 +63,9 @@ def _plain_call(norm) -> bool:
 
 
 def _add_norm(norm, x, residual):
-    """``(norm(h), h)`` with h = x + residual: one fused call, or a sum and a call of the module where that does more than its forward."""
-    if _plain_call(norm):
+    """``(norm(h), h)`` with h = x + residual: one fused call, or a sum and a call of the module where that does more than its forward
+    or the two types differ (autocast: a 16-bit attention output on an fp32 stream, which torch adds in fp32)."""
+    if _plain_call(norm) and (residual is None or residual.dtype == x.dtype):
         return add_rms_norm(x, residual, _weight_for(norm, x), norm.variance_epsilon)
     h = x if residual is None else residual + x
     return norm(h), h

@@ -127,3 +127,9 @@ def test_global_hooks_backward_hooks_and_replaced_forwards_run(patched):
     assert not torch.allclose(_both_own, layer(x))
     layer.input_layernorm = torch.nn.Identity()                        # another module in its place
     _both(layer, x, patched)
+
+
+@pytest.mark.parametrize("dtype,attention", [(torch.float32, torch.bfloat16), (torch.float32, torch.float16)])
+def test_a_stream_wider_than_the_attention_s_output(patched, dtype, attention):
+    layer, x = _layer(dtype, attention)
+    assert _both(layer, x, patched).dtype == torch.float32
