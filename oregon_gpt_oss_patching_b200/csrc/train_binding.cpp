@@ -330,9 +330,12 @@ std::pair<Tensor, Tensor> router_topk(const Tensor& logits, int64_t top_k, const
   TORCH_CHECK_VALUE(top_k >= 1 && top_k <= std::min<int64_t>(B200MOE_ROUTER_MAX_TOP_K, eligible), "router_topk: cannot choose ", top_k, " of ",
                     eligible, " eligible experts (at most ", B200MOE_ROUTER_MAX_TOP_K, ")");
   TORCH_CHECK_VALUE(logits.size(0) <= std::numeric_limits<int32_t>::max(), "router_topk: ", logits.size(0), " tokens");
-  if (bias.has_value())
+  if (bias.has_value()) {
     TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == experts && bias->device() == logits.device() && bias->is_floating_point(),
                       "router_topk: bias must be ", experts, " floating point values on ", logits.device());
+    // (the kernels read it as fp32, where every value of these types is itself)
+    TORCH_CHECK_TYPE(dtype_code(bias->scalar_type()) >= 0, "router_topk: bias must be bfloat16, float16 or float32, got ", bias->dtype());
+  }
   check_no_tangent("router_topk", logits, bias);
   const Routing how{top_k, num_groups, top_groups, scoring == "sigmoid", renormalize, scale};
   const bool differentiable = at::GradMode::is_enabled() && logits.requires_grad();

@@ -26,8 +26,8 @@ def router_topk(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", b
     """``(weights, indices)`` of the ``top_k`` experts of every token, both (tokens, top_k), best first.
 
     logits (tokens, experts): bf16, fp16 or fp32, at most 256 experts; weights have the logits' type, indices are int64, as
-    ``moe_experts`` takes them.  ``scoring`` is "softmax" (over all experts) or "sigmoid"; ``bias`` (experts) is added to the scores
-    for the choice alone and gets no gradient; with ``num_groups`` only the experts of the ``top_groups`` groups with the
+    ``moe_experts`` takes them.  ``scoring`` is "softmax" (over all experts) or "sigmoid"; ``bias`` (experts; bf16, fp16 or fp32)
+    is added to the scores for the choice alone and gets no gradient; with ``num_groups`` only the experts of the ``top_groups`` groups with the
     largest sums of their two best values are eligible; ``renormalize`` divides the weights by their sum; ``scale`` multiplies them.
     """
     return _binding.load().router_topk(logits, top_k, scoring, bias, num_groups, num_groups if top_groups is None else top_groups, renormalize, scale)

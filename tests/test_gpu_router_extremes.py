@@ -89,3 +89,13 @@ def test_an_infinite_logit_does_not_open_a_masked_group(groups, top_groups, with
     assert torch.equal(i.cpu(), ref)
     if top_groups < groups:
         assert bool((i >= size).all())
+
+
+def test_a_bias_keeps_all_its_bits():
+    l = torch.randn(5, 32, device=DEV)
+    with pytest.raises(TypeError, match="bias"):
+        router_topk(l, 4, scoring="sigmoid", bias=torch.zeros(32, device=DEV, dtype=torch.float64))
+    for dtype in (BF16, FP16, FP32):
+        b = (torch.randn(32, generator=torch.Generator().manual_seed(6)) * 0.1).to(device=DEV, dtype=dtype)
+        _, i = router_topk(l, 4, scoring="sigmoid", bias=b)
+        assert torch.equal(i, step_fp64.router_topk(l, 4, sigmoid=True, bias=b)[1])
