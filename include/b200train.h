@@ -66,8 +66,9 @@ int b200train_add_rms_norm_bwd(const void* dy, int64_t dy_stride, const void* dh
  *                                   aligned), elements (>= 0), element types.  A tensor's elements are contiguous; no two
  *                                   tensors of a call that writes may overlap (B200TRAIN_EOVERLAP).
  *   scratch                         device fp64, b200train_clip_scratch_doubles(...) of them
- *   norm                            out, device fp32: n = sqrt(sum of g^2 over all tensors).  Squares are fp32, sums beyond a
- *                                   few hundred of them fp64: an element above 1.8e19 makes n infinite.
+ *   norm                            out, device fp32: n = sqrt(sum of g^2 over all tensors).  Squares are fp32, their sums
+ *                                   fp32 within 16 bytes of a tensor and fp64 beyond (n is right to 2.5 * 2^-24): an element
+ *                                   above 1.8e19, or a few of 16 bytes near it, makes n infinite.
  * c = min(1, max_norm / (n + 1e-6)), max_norm >= 0; a NaN norm makes c NaN, an infinite one 0; max_norm = inf is no limit, c = 1.
  * No value is read by the host.
  */

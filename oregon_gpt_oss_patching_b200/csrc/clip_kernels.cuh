@@ -100,12 +100,30 @@ struct Chunk {
 constexpr int kBatch = 4;
 static_assert(kChunkWords % (kClipThreads * kBatch) == 0, "a whole chunk is whole batches");
 
+// The sum of the squares of a 16-byte word's elements.  It is made in fp32, a tree of two (fp32 elements) or three additions, and all
+// above it in fp64: the sum is right to 3 * 2^-24 whatever the sizes and the order of its terms.  (fp64 from the squares on, which is
+// 2^-24 for fp32 elements and exact for others, is bound by the conversions: 823 M bf16 237 to 241 us instead of 232, 20 M in L2 12.9
+// instead of 9.2.  fp32 for all of a thread's words in a chunk, up to 64 squares, costs the same as this and may be off by 64 * 2^-24.)
+template <int N>
+__device__ __forceinline__ double word_sumsq(const F2 (&f)[N / 2]) {
+  F2 p[N / 2];
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) p[e] = mul2(f[e], f[e]);
+#pragma unroll
+  for (int n = N / 4; n > 0; n /= 2) {
+#pragma unroll
+    for (int e = 0; e < n; ++e) p[e] = add2(p[e], p[e + n]);
+  }
+  const float2 s = split2(p[0]);
+  return (double)(s.x + s.y);
+}
+
 template <typename T>
-__device__ __forceinline__ float chunk_sumsq(const void* grad, long long count, unsigned index) {
+__device__ __forceinline__ double chunk_sumsq(const void* grad, long long count, unsigned index) {
   constexpr int N = Elem<T>::N;
   const Chunk<T> c(grad, count, index);
   const T* g = static_cast<const T*>(grad);
-  F2 sum = 0;
+  double sum = 0.0;
   if (c.whole()) {
     const uint4* w = reinterpret_cast<const uint4*>(g + c.at(c.begin, 0)) + threadIdx.x;
     uint4 v[kChunkWords / kClipThreads];
@@ -115,36 +133,32 @@ __device__ __forceinline__ float chunk_sumsq(const void* grad, long long count, 
     for (int i = 0; i < kChunkWords / kClipThreads; ++i) {
       F2 f[N / 2];
       unpack<T>(v[i], f);
-#pragma unroll
-      for (int e = 0; e < N / 2; ++e) sum = fma2(f[e], f[e], sum);
+      sum += word_sumsq<N>(f);
     }
   } else {
     for (long long w = c.begin + threadIdx.x; w < c.end; w += kClipThreads) {
       float f[N];
       c.load(g, w, true, f);
+      F2 pairs[N / 2];
 #pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        const F2 p = make2(f[e], f[e + 1]);
-        sum = fma2(p, p, sum);
-      }
+      for (int e = 0; e < N; e += 2) pairs[e / 2] = make2(f[e], f[e + 1]);
+      sum += word_sumsq<N>(pairs);
     }
   }
-  const float2 s = split2(sum);
-  return s.x + s.y;
+  return sum;
 }
 
-// A thread's sum over a chunk is fp32 (a few hundred terms), everything above it fp64.
 __global__ void __launch_bounds__(kClipThreads) grad_sumsq_kernel(const __grid_constant__ ClipTable t, double* partials) {
   asm volatile("griddepcontrol.launch_dependents;");
   double sum = 0.0;
   for (unsigned chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
     const int i = tensor_of(t, chunk);
     const unsigned index = chunk - t.first[i];
-    float s;
+    double s;
     if (t.dtype[i] == 0) s = chunk_sumsq<__nv_bfloat16>(t.grad[i], t.count[i], index);
     else if (t.dtype[i] == 1) s = chunk_sumsq<__half>(t.grad[i], t.count[i], index);
     else s = chunk_sumsq<float>(t.grad[i], t.count[i], index);
-    sum += (double)s;
+    sum += s;
   }
   sum = block_sum(sum);
   if (threadIdx.x == 0) partials[blockIdx.x] = sum;
