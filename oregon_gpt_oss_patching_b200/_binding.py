@@ -29,10 +29,11 @@ def load():
     with _lock:
         if _module is not None:
             return _module
-        if not os.path.exists(_build.BINDING_PATH):
-            raise RuntimeError(f"{_build.BINDING_PATH} not found: the extension module has not been built "
+        path = _build.binding_path()
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} not found: the extension module has not been built "
                                "(run `python -m oregon_gpt_oss_patching_b200.build`); there is no fallback path")
-        loader = importlib.machinery.ExtensionFileLoader("_train_binding", _build.BINDING_PATH)
+        loader = importlib.machinery.ExtensionFileLoader("_train_binding", path)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_train_binding", loader))
         loader.exec_module(module)
         module.set_library({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _NAMES})
