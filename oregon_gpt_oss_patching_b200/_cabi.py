@@ -55,8 +55,6 @@ class Params(ctypes.Structure):
 
 
 MOE_ROW_ALIGN = 128          # B200MOE_ROW_ALIGN
-MOE_ROUTER_MAX_EXPERTS, MOE_ROUTER_MAX_TOP_K, MOE_ROUTER_MAX_GROUPS = 256, 32, 32   # B200MOE_ROUTER_MAX_*
-MOE_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # B200MOE_BF16, _FP16, _FP32
 MOE_ROWS_NN, MOE_ROWS_NT, MOE_INNER_TN = 0, 1, 2
 
 

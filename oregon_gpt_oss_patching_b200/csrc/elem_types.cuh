@@ -53,7 +53,6 @@ struct Elem<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-  static __device__ __forceinline__ float round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
 };
 
 template <>
@@ -70,7 +69,6 @@ struct Elem<__half> {
   }
   static __device__ __forceinline__ float load1(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
-  static __device__ __forceinline__ float round(float v) { return __half2float(__float2half_rn(v)); }
 };
 
 template <>
@@ -78,7 +76,6 @@ struct Elem<float> {
   static constexpr int N = 4;
   static __device__ __forceinline__ float load1(const float* p) { return *p; }
   static __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
-  static __device__ __forceinline__ float round(float v) { return v; }
 };
 
 template <typename T>
