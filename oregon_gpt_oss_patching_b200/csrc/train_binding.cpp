@@ -91,6 +91,8 @@ int dtype_code(at::ScalarType t) {
 
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
 bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+// A tensor whose memory holds its values: the imaginary part of a conjugate, for one, is a view that torch negates where it reads it.
+Tensor as_it_lies(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 Tensor copy_of(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
 // A contiguous tensor on x's device, without the dispatcher's way there (half the time of at::empty, and most calls make two to five).
 Tensor empty_on(const Tensor& x, at::IntArrayRef sizes, at::ScalarType type) {
@@ -105,7 +107,7 @@ struct Rows {
   Tensor t;
   int64_t stride;
   Rows() : stride(0) {}
-  Rows(const Tensor& of, int64_t cols) : t(of), stride(cols) {
+  Rows(const Tensor& of, int64_t cols) : t(as_it_lies(of)), stride(cols) {
     if (!t.is_contiguous()) {
       t = t.reshape({-1, cols});
       const int64_t per_word = 16 / static_cast<int64_t>(t.element_size());
@@ -139,7 +141,7 @@ void check_norm(const char* name, const Tensor& x, const std::optional<Tensor>& 
 }
 
 // A weight as the kernels read it: contiguous, on the 16-byte grid.
-Tensor on_grid(const Tensor& w) { return w.is_contiguous() && aligned16(w) ? w : copy_of(w); }
+Tensor on_grid(const Tensor& w) { return w.is_contiguous() && !w.is_neg() && aligned16(w) ? w : copy_of(w); }
 
 // A saved value that comes back through a hook (an offload, a compression) may lie otherwise in memory than it did: each is laid
 // out for the kernels again, once it is known to be what was saved.
@@ -273,7 +275,7 @@ std::pair<Tensor, Tensor> router_forward(const Tensor& logits, const std::option
   const int device = logits.get_device();
   const int64_t tokens = logits.size(0), experts = logits.size(1);
   Tensor b;
-  if (bias.has_value()) b = bias->to(at::kFloat).contiguous();
+  if (bias.has_value()) b = as_it_lies(bias->to(at::kFloat)).contiguous();
   Tensor weights = empty_on(logits, {tokens, how.top_k}, logits.scalar_type());
   Tensor indices = empty_on(logits, {tokens, how.top_k}, at::kLong);
   check(lib.router_topk(data(logits), logits.stride(0), b.defined() ? b.const_data_ptr<float>() : nullptr, weights.mutable_data_ptr(),
@@ -285,7 +287,10 @@ std::pair<Tensor, Tensor> router_forward(const Tensor& logits, const std::option
 }
 
 // A row's elements lie next to each other.
-Tensor row_major(const Tensor& logits) { return logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous(); }
+Tensor row_major(const Tensor& logits) {
+  const Tensor l = as_it_lies(logits);
+  return l.stride(1) == 1 || l.size(1) == 1 ? l : l.contiguous();
+}
 
 struct RouterTopkBackward : Node {
   SavedVariable logits, indices;
@@ -301,7 +306,7 @@ struct RouterTopkBackward : Node {
   variable_list apply(variable_list&& grads) override {
     TORCH_CHECK(!at::GradMode::is_enabled(), "router_topk cannot be differentiated twice");
     if (!grads[0].defined()) return {Tensor()};
-    const Tensor dweights = grads[0].contiguous(), saved = logits.unpack(), saved_indices = indices.unpack();
+    const Tensor dweights = as_it_lies(grads[0]).contiguous(), saved = logits.unpack(), saved_indices = indices.unpack();
     check_saved("router_topk", saved, {dweights.size(0), experts}, dweights.scalar_type(), dweights.device());
     check_saved("router_topk", saved_indices, dweights.sizes(), at::kLong, dweights.device());
     const Tensor l = row_major(saved), chosen = saved_indices.contiguous();
@@ -481,7 +486,7 @@ struct Output {
   }
 };
 
-Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+Tensor dense(const Tensor& t) { return t.is_neg() ? t.resolve_neg().contiguous() : t.is_contiguous() ? t : t.contiguous(); }
 
 float limit_of(const char* name, double max_norm) {
   TORCH_CHECK_VALUE(max_norm >= 0.0, name, ": max_norm must not be negative, got ", max_norm);
