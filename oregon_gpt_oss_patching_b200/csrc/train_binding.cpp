@@ -438,10 +438,26 @@ void check_apart(const char* name, const std::vector<Tensor>& written, const std
       TORCH_CHECK_VALUE(t.stride(d) != 0 || t.size(d) <= 1, name, ": a tensor with a stride of 0 cannot be written in place");
     TORCH_CHECK_VALUE(!shares_with_itself(Span(t)), name, ": a tensor whose elements share memory cannot be written in place");
   }
-  std::vector<std::pair<Span, bool>> all;
-  all.reserve(written.size() + read.size());
-  for (const Tensor& t : written) all.emplace_back(Span(t), true);
-  for (const Tensor& t : read) all.emplace_back(Span(t), false);
+  std::vector<std::pair<Span, bool>> all;   // and whether it is written
+  int64_t low = std::numeric_limits<int64_t>::max(), high = 0;
+  const auto strided = [&](const std::vector<Tensor>& tensors, bool writes) {
+    for (const Tensor& t : tensors) {
+      if (t.is_contiguous()) continue;
+      all.emplace_back(Span(t), writes);
+      low = std::min(low, all.back().first.begin);
+      high = std::max(high, all.back().first.begin + all.back().first.bytes);
+    }
+  };
+  strided(written, true);
+  strided(read, false);
+  const auto near = [&](const std::vector<Tensor>& tensors, bool writes) {   // contiguous ones that one of those could reach
+    for (const Tensor& t : tensors) {
+      const int64_t begin = reinterpret_cast<int64_t>(t.const_data_ptr());
+      if (t.is_contiguous() && begin < high && begin + t.numel() * static_cast<int64_t>(t.element_size()) > low) all.emplace_back(Span(t), writes);
+    }
+  };
+  near(written, true);
+  near(read, false);
   std::sort(all.begin(), all.end(), [](const auto& a, const auto& b) { return a.first.begin < b.first.begin; });
   for (size_t i = 0; i < all.size(); ++i)
     for (size_t j = i + 1; j < all.size() && all[j].first.begin < all[i].first.begin + all[i].first.bytes; ++j)
