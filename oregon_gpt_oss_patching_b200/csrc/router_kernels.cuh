@@ -291,7 +291,17 @@ __device__ __forceinline__ void merge_keys(uint32_t (&a)[LL], const uint32_t (&b
 
 // Sigmoid scores as numbers: s = e^min(x,0) / (1 + e^-|x|) over e^shift.  Shares s_j / sum_S s do not depend on the shift, and with the
 // largest chosen logit m in it, where that is negative, they are right however low the logits lie (e^-89 is no fp32 number).
-__device__ __forceinline__ float share_shift(float m) { return m < 0.f && m != -CUDART_INF_F ? m : 0.f; }
+// (The maximum over the lanes that serve a token: one instruction where that is the whole warp.)
+__device__ __forceinline__ float share_shift(float x, int width) {
+  float m;
+  if (width == 32) {
+    const uint32_t key = __reduce_max_sync(0xffffffffu, order_key(x));
+    m = key >= order_key(0.f) ? 0.f : __uint_as_float(~key);
+  } else {
+    m = lanes_max(x, width);
+  }
+  return m < 0.f && m != -CUDART_INF_F ? m : 0.f;
+}
 __device__ __forceinline__ float sigmoid_over(float x, float shift) { return expf(fminf(x, 0.f) - shift) / (1.f + expf(-fabsf(x))); }
 
 // The weights of the elected: lane j (of `width` that serve the token) has the j-th expert and its logit x, `chosen` for
@@ -300,7 +310,7 @@ template <typename T>
 __device__ __forceinline__ void write_choice(const RouterArgs& a, long long at, bool chosen, int width, int expert, float x, float m, float z) {
   float s;
   if (a.sigmoid) {
-    const float shift = a.renormalize ? share_shift(lanes_max(chosen ? x : -CUDART_INF_F, width)) : 0.f;
+    const float shift = a.renormalize ? share_shift(chosen ? x : -CUDART_INF_F, width) : 0.f;
     s = chosen ? sigmoid_over(x, shift) : 0.f;
   } else {
     if (a.renormalize) m = lanes_max(chosen ? x : -CUDART_INF_F, width);
@@ -530,7 +540,7 @@ __global__ void __launch_bounds__(kRouterThreads) router_topk_bwd_kernel(const _
   if (a.sigmoid) {
     const float x = expf(-fabsf(lj)), rest = (lj >= 0.f ? x : 1.f) / (1.f + x);   // 1 - s (no overflow on either side)
     if (a.renormalize) {
-      const float s = sigmoid_over(lj, share_shift(lanes_max(lj, W)));   // (0 where there is no expert)
+      const float s = sigmoid_over(lj, share_shift(lj, W));   // (0 where there is no expert)
       const float sum = lanes_add(s, W);
       const float r = sum == 0.f ? 0.f : s / sum;
       chosen = r * (d - lanes_add(e >= 0 ? d * r : 0.f, W)) * rest;
