@@ -90,7 +90,20 @@ int dtype_code(at::ScalarType t) {
 }
 
 void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
-bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+// A tensor's address.  Fake tensors and wrappers of others pass for CUDA tensors and have no memory of their own; an offset into
+// nothing would be an address like any other.
+const void* address(const Tensor& t) {
+  TORCH_CHECK(t.numel() == 0 || t.storage().data() != nullptr, "needs tensors with memory of their own, got one without (a fake tensor or a wrapper)");
+  return t.const_data_ptr();
+}
+template <typename... T>
+void check_memory(const T&... tensors) {
+  const auto look = [](const std::optional<Tensor>& t) {
+    if (t.has_value()) address(*t);
+  };
+  (look(tensors), ...);
+}
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(address(t)) % 16 == 0; }
 // A tensor whose memory holds its values: the imaginary part of a conjugate, for one, is a view that torch negates where it reads it.
 Tensor as_it_lies(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 Tensor copy_of(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); }
@@ -98,7 +111,7 @@ Tensor copy_of(const Tensor& t) { return t.clone(at::MemoryFormat::Contiguous); 
 Tensor empty_on(const Tensor& x, at::IntArrayRef sizes, at::ScalarType type) {
   return at::detail::empty_cuda(sizes, type, x.device(), std::nullopt);
 }
-const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+const void* data(const Tensor& t) { return t.defined() ? address(t) : nullptr; }
 
 // ---------------------------------------------------------------- norm
 
@@ -137,6 +150,7 @@ void check_norm(const char* name, const Tensor& x, const std::optional<Tensor>& 
                       residual->dtype(), ", ", residual->device());
   TORCH_CHECK_VALUE(eps >= 0.0, name, ": eps must not be negative, got ", eps);
   TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int32_t>::max(), name, ": rows of ", x.size(-1), " elements");
+  check_memory(x, residual, weight);
   check_no_tangent(name, x, residual, weight);
 }
 
@@ -278,7 +292,7 @@ std::pair<Tensor, Tensor> router_forward(const Tensor& logits, const std::option
   if (bias.has_value()) b = as_it_lies(bias->to(at::kFloat)).contiguous();
   Tensor weights = empty_on(logits, {tokens, how.top_k}, logits.scalar_type());
   Tensor indices = empty_on(logits, {tokens, how.top_k}, at::kLong);
-  check(lib.router_topk(data(logits), logits.stride(0), b.defined() ? b.const_data_ptr<float>() : nullptr, weights.mutable_data_ptr(),
+  check(lib.router_topk(data(logits), logits.stride(0), static_cast<const float*>(data(b)), weights.mutable_data_ptr(),
                         indices.mutable_data_ptr<int64_t>(), static_cast<int32_t>(tokens), static_cast<int32_t>(experts),
                         static_cast<int32_t>(how.top_k), static_cast<int32_t>(how.num_groups), static_cast<int32_t>(how.top_groups), how.sigmoid,
                         how.renormalize, static_cast<float>(how.scale), dtype_code(logits.scalar_type()), device, stream_of(device)),
@@ -312,7 +326,7 @@ struct RouterTopkBackward : Node {
     const Tensor l = row_major(saved), chosen = saved_indices.contiguous();
     const int device = l.get_device();
     Tensor dlogits = empty_on(l, l.sizes(), l.scalar_type());
-    check(lib.router_topk_bwd(data(l), l.stride(0), chosen.const_data_ptr<int64_t>(), data(dweights), dlogits.mutable_data_ptr(),
+    check(lib.router_topk_bwd(data(l), l.stride(0), static_cast<const int64_t*>(data(chosen)), data(dweights), dlogits.mutable_data_ptr(),
                               static_cast<int32_t>(l.size(0)), static_cast<int32_t>(l.size(1)), static_cast<int32_t>(chosen.size(1)), sigmoid,
                               renormalize, static_cast<float>(scale), dtype_code(l.scalar_type()), device, stream_of(device)),
           "b200moe_router_topk_bwd");
@@ -341,6 +355,7 @@ std::pair<Tensor, Tensor> router_topk(const Tensor& logits, int64_t top_k, const
     // (the kernels read it as fp32, where every value of these types is itself)
     TORCH_CHECK_TYPE(dtype_code(bias->scalar_type()) >= 0, "router_topk: bias must be bfloat16, float16 or float32, got ", bias->dtype());
   }
+  check_memory(logits, bias);
   check_no_tangent("router_topk", logits, bias);
   const Routing how{top_k, num_groups, top_groups, scoring == "sigmoid", renormalize, scale};
   const bool differentiable = at::GradMode::is_enabled() && logits.requires_grad();
@@ -486,8 +501,8 @@ struct Table {
       dtypes[i] = dtype_code(g[i].scalar_type());
       TORCH_CHECK_TYPE(dtypes[i] >= 0, name, " supports bfloat16, float16 and float32, got ", g[i].dtype());
       counts[i] = g[i].numel();
-      grads[i] = reinterpret_cast<int64_t>(g[i].const_data_ptr());
-      if (p != nullptr) params[i] = reinterpret_cast<int64_t>((*p)[i].const_data_ptr());
+      grads[i] = reinterpret_cast<int64_t>(address(g[i]));
+      if (p != nullptr) params[i] = reinterpret_cast<int64_t>(address((*p)[i]));
     }
   }
 };
