@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -75,6 +76,10 @@ bool has_tangent(const std::optional<Tensor>& t) { return t.has_value() && has_t
 template <typename... T>
 void check_no_tangent(const char* name, const T&... tensors) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(tensors) || ...), name, " has no forward-mode derivative");
+}
+// A trace would keep this call's results as constants.
+void check_not_traced(const char* name) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), name, " cannot be traced: the trace would keep its results for these inputs");
 }
 // Whether any tensor can have a tangent: asked once where there are many of them.
 bool tangents_exist() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
@@ -150,6 +155,7 @@ void check_norm(const char* name, const Tensor& x, const std::optional<Tensor>& 
                       residual->dtype(), ", ", residual->device());
   TORCH_CHECK_VALUE(eps >= 0.0, name, ": eps must not be negative, got ", eps);
   TORCH_CHECK_VALUE(x.size(-1) <= std::numeric_limits<int32_t>::max(), name, ": rows of ", x.size(-1), " elements");
+  check_not_traced(name);
   check_memory(x, residual, weight);
   check_no_tangent(name, x, residual, weight);
 }
@@ -355,6 +361,7 @@ std::pair<Tensor, Tensor> router_topk(const Tensor& logits, int64_t top_k, const
     // (the kernels read it as fp32, where every value of these types is itself)
     TORCH_CHECK_TYPE(dtype_code(bias->scalar_type()) >= 0, "router_topk: bias must be bfloat16, float16 or float32, got ", bias->dtype());
   }
+  check_not_traced("router_topk");
   check_memory(logits, bias);
   check_no_tangent("router_topk", logits, bias);
   const Routing how{top_k, num_groups, top_groups, scoring == "sigmoid", renormalize, scale};
@@ -526,6 +533,7 @@ float limit_of(const char* name, double max_norm) {
 
 Tensor global_grad_norm(const std::vector<Tensor>& tensors) {
   at::NoGradGuard no_grad;
+  check_not_traced("global_grad_norm");
   if (tensors.empty()) return at::zeros({}, at::kFloat);
   std::vector<Tensor> packed;
   packed.reserve(tensors.size());
@@ -544,6 +552,7 @@ Tensor global_grad_norm(const std::vector<Tensor>& tensors) {
 
 Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm) {
   at::NoGradGuard no_grad;
+  check_not_traced("clip_grad_norm");
   const float limit = limit_of("clip_grad_norm", max_norm);
   std::vector<Tensor> grads, packed;
   const bool tangents = tangents_exist();
@@ -574,6 +583,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm) {
 
 Tensor clipped_sgd_step(const std::vector<Tensor>& parameters, double lr, double max_norm) {
   at::NoGradGuard no_grad;
+  check_not_traced("clipped_sgd_step");
   const float limit = limit_of("clipped_sgd_step", max_norm);
   std::vector<Tensor> params, grads, packed;
   const bool tangents = tangents_exist();
