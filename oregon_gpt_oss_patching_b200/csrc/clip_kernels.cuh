@@ -4,8 +4,9 @@
 //
 // Two launches: `grad_sumsq_kernel` reads every gradient once and leaves one partial sum a CTA; each CTA of the second
 // kernel adds the same partials in the same order, so all of them hold the same c without a third launch, a counter or
-// atomics, and writes back (nothing, where c = 1).  The second may start while the first runs out, and goes through the
-// tensors backwards: what the first read last is still in L2.
+// atomics, and writes back (nothing, where c = 1).  The second may start while the first runs out, and goes through its
+// tensors backwards, since what the first read last is still in L2.  (Lists of more than kClipTensors take a launch of each kernel for every
+// so many, in the list's order; of those only the last launch's tensors can still be there.)
 //
 // Both are bound by HBM: clipping cannot do without reading the gradients twice (unless they fit in L2) and writing them once;
 // the folded update reads gradients twice and parameters once and writes the parameters, where clipping first and updating

@@ -12,7 +12,7 @@
 // experts (whole lanes to a group) into keys: the upper 24 bits of the value in an order of unsigned integers, and 255 - expert
 // below, so that keys differ and the larger one is the one to elect.  It sorts them by eights with a network, keeps the best 8
 // (or 4, where top_k allows), and three exchanges between the lanes leave the token's best in all of them.  Instructions bound
-// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 37 us forward (26 us
+// the kernel, not memory (a few MB): 32771 tokens, 8 of 256 experts, sigmoid, bias, 4 of 8 groups take 38 us forward (26 us
 // without the doubtful tokens, below), on logits alone 12.5 us, and 8 us backward.  (A warp a token with a warp-wide maximum a
 // round: 66, 25 and 12 us; that with full keys, two maxima a round and groups summed through shared memory: 89 and 37 us.)
 //
