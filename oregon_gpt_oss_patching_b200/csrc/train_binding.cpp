@@ -451,31 +451,36 @@ bool shares_with_itself(const Span& t) {
   return false;
 }
 
-// Refuses tensors to be written that have memory twice, share it with one another or with one that is read.  Contiguous tensors are
-// looked through by the library; where there are others it sees copies of them.
+// Whether the library gets a tensor itself; otherwise a copy, which dense() makes.
+bool goes_itself(const Tensor& t) { return t.is_contiguous() && !t.is_neg(); }
+Tensor dense(const Tensor& t) { return goes_itself(t) ? t : as_it_lies(t).contiguous(); }
+
+// Refuses tensors to be written that have memory twice, share it with one another or with one that is read.  What goes to the library
+// itself is looked through there.
 void check_apart(const char* name, const std::vector<Tensor>& written, const std::vector<Tensor>& read) {
   for (const Tensor& t : written) {
-    if (t.is_contiguous()) continue;
+    if (goes_itself(t)) continue;
     for (int64_t d = 0; d < t.dim(); ++d)
       TORCH_CHECK_VALUE(t.stride(d) != 0 || t.size(d) <= 1, name, ": a tensor with a stride of 0 cannot be written in place");
     TORCH_CHECK_VALUE(!shares_with_itself(Span(t)), name, ": a tensor whose elements share memory cannot be written in place");
   }
   std::vector<std::pair<Span, bool>> all;   // and whether it is written
   int64_t low = std::numeric_limits<int64_t>::max(), high = 0;
-  const auto strided = [&](const std::vector<Tensor>& tensors, bool writes) {
+  const auto copied = [&](const std::vector<Tensor>& tensors, bool writes) {
     for (const Tensor& t : tensors) {
-      if (t.is_contiguous()) continue;
+      if (goes_itself(t)) continue;
       all.emplace_back(Span(t), writes);
+      if (t.numel() == 0) continue;
       low = std::min(low, all.back().first.begin);
       high = std::max(high, all.back().first.begin + all.back().first.bytes);
     }
   };
-  strided(written, true);
-  strided(read, false);
-  const auto near = [&](const std::vector<Tensor>& tensors, bool writes) {   // contiguous ones that one of those could reach
+  copied(written, true);
+  copied(read, false);
+  const auto near = [&](const std::vector<Tensor>& tensors, bool writes) {   // and the others that one of those could reach
     for (const Tensor& t : tensors) {
       const int64_t begin = reinterpret_cast<int64_t>(t.const_data_ptr());
-      if (t.is_contiguous() && begin < high && begin + t.numel() * static_cast<int64_t>(t.element_size()) > low) all.emplace_back(Span(t), writes);
+      if (goes_itself(t) && begin < high && begin + t.numel() * static_cast<int64_t>(t.element_size()) > low) all.emplace_back(Span(t), writes);
     }
   };
   near(written, true);
@@ -523,8 +528,6 @@ struct Output {
     norm = empty_on(like, {}, at::kFloat);
   }
 };
-
-Tensor dense(const Tensor& t) { return t.is_neg() ? t.resolve_neg().contiguous() : t.is_contiguous() ? t : t.contiguous(); }
 
 float limit_of(const char* name, double max_norm) {
   TORCH_CHECK_VALUE(max_norm >= 0.0, name, ": max_norm must not be negative, got ", max_norm);

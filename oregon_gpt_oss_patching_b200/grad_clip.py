@@ -30,7 +30,7 @@ def _listed(tensors: _Tensors) -> list:
 
 
 def global_grad_norm(tensors: _Tensors) -> torch.Tensor:
-    """The 2-norm of all the tensors' elements together, an fp32 scalar on their device (0 on the CPU for no tensors)."""
+    """The 2-norm of all the tensors' elements together, an fp32 scalar on their device (0 on the CPU for no tensors), without a gradient."""
     return _binding.load().global_grad_norm(_listed(tensors))
 
 

@@ -49,3 +49,14 @@ def test_gradients_of_a_complex_product():
     q.grad = torch.full((8,), 0.5, device=DEV)
     clipped_sgd_step([q], 1.0)
     assert q.tolist() == [0.5] * 8
+
+
+def test_a_negated_gradient_given_twice_is_refused():
+    p = torch.nn.Parameter(torch.ones(8, device=DEV))
+    p.grad = negated(torch.full((8,), 0.5, device=DEV))
+    other = torch.nn.Parameter(torch.ones(8, device=DEV))
+    other.grad = torch.ones(8, device=DEV)
+    for call in (lambda: clip_grad_norm([other, p, p], 0.1), lambda: clipped_sgd_step([p, other, p], 0.1)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            call()
+    assert p.tolist() == other.tolist() == [1.0] * 8 and p.grad.tolist() == [0.5] * 8
